@@ -67,6 +67,10 @@ SYMBOLS = {
                                     C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     "f5hip_reset_kernel_stats": (C.c_int, [_P]),
     "f5hip_attention_stats": (C.c_int, [_P, C.POINTER(C.c_double), C.c_int]),
+    "f5hip_rotary_frequencies": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_int64, C.c_double, C.c_double, _P, C.POINTER(C.c_double)]),
+    "f5hip_rotary": (C.c_int, [_P, C.c_int, _P]),
+    "f5hip_window_attention_workspace": (C.c_int64, [_P]),
+    "f5hip_window_attention": (C.c_int, [_P, C.c_int, _P]),
     "f5hip_bigvgan_create": (C.c_int, [C.POINTER(BigVGANConfigC), C.c_int, C.POINTER(_P)]),
     "f5hip_bigvgan_destroy": (C.c_int, [_P]),
     "f5hip_bigvgan_last_error": (C.c_char_p, [_P]),

@@ -1664,6 +1664,16 @@ extern "C" {
 
 int f5hip_abi_version(void) { return F5HIP_ABI_VERSION; }
 
+}  // extern "C"
+// the text f5hip_last_error(NULL) returns on this thread; for the entry points without a context (operators_api.cpp).  Returns `code`.
+int f5hip_set_thread_error(int code, const char* text) {
+  try {
+    g_create_err = text;
+  } catch (...) {  // out of memory: the code is all there is
+  }
+  return code;
+}
+extern "C" {
 const char* f5hip_last_error(const f5hip_ctx* ctx) { return ctx ? ctx->err.c_str() : g_create_err.c_str(); }
 
 int f5hip_create(const f5hip_dit_config* dc, const f5hip_vocos_config* vc, int device, f5hip_ctx** out) {

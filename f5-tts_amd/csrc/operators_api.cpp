@@ -1,0 +1,159 @@
+// operators_api.cpp — entry points of the operators (include/f5hip.h, "operators"): argument checks, device guard, per-thread error text.
+#include <cmath>
+#include <cstdio>
+
+#include "operators.h"
+#ifndef F5_HIPEMU
+#include <hip/hip_runtime.h>
+#endif
+
+int f5hip_set_thread_error(int code, const char* text);  // api.cpp: the text f5hip_last_error(NULL) returns
+
+namespace {
+int elt_bytes(int dtype) { return dtype == F5HIP_T_FP32 ? 4 : 2; }
+
+// |any element offset| of a [batch, tokens, heads, dim] tensor stays far below 2^63, so the kernels' 64-bit offsets cannot wrap
+bool strides_ok(const int64_t (&st)[3], const int64_t (&ext)[3], bool output) {
+  for (int i = 0; i < 3; ++i) {
+    if (st[i] < 0 || st[i] > (int64_t(1) << 40)) return false;
+    if (output && st[i] == 0 && ext[i] > 1) return false;
+  }
+  return true;
+}
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// the calling thread's device while an operator launches, restored on every path
+struct DeviceGuard {
+  int before = -1;
+  bool changed = false;
+  hipError_t enter(int device) {
+    hipError_t e = hipGetDevice(&before);
+    if (e != hipSuccess || before == device) return e;
+    e = hipSetDevice(device);
+    changed = e == hipSuccess;
+    return e;
+  }
+  ~DeviceGuard() {
+    if (changed) (void)hipSetDevice(before);
+  }
+};
+
+template <typename F>
+int on_device(int device, F&& launch) {
+  int n = 0;
+  if (hipGetDeviceCount(&n) != hipSuccess || n == 0) return f5hip_set_thread_error(F5HIP_ERR_HIP, "no HIP device: there is no CPU fallback");
+  if (device < 0 || device >= n) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "device ordinal out of range");
+  DeviceGuard guard;
+  hipError_t e = guard.enter(device);
+  if (e == hipSuccess) e = launch();
+  if (e == hipSuccess) return F5HIP_OK;
+  char b[128];
+  snprintf(b, sizeof(b), "operator launch failed: %s", hipGetErrorString(e));
+  return f5hip_set_thread_error(F5HIP_ERR_HIP, b);
+}
+}  // namespace
+
+const char* check_rotary(const f5hip_rotary_args& a) {
+  if (a.dtype < F5HIP_T_FP32 || a.dtype > F5HIP_T_BF16) return "rotary: dtype must be fp32, fp16 or bf16";
+  if (a.layout != F5HIP_ROTARY_INTERLEAVED && a.layout != F5HIP_ROTARY_HALF) return "rotary: unknown layout";
+  if (a.batch < 0 || a.tokens < 0 || a.heads_q < 1 || a.heads_k < 0 || a.head_dim < 2) return "rotary: batch, tokens >= 0, heads_q >= 1, heads_k >= 0, head_dim >= 2";
+  if (a.rot_dim < 2 || (a.rot_dim & 1) || a.rot_dim > a.head_dim) return "rotary: rot_dim must be even and in [2, head_dim]";
+  if (a.rot_heads < -1) return "rotary: rot_heads must be -1 (all) or a number of heads";
+  if (a.head_dim > 4096 || a.heads_q > 65536 || a.heads_k > 65536) return "rotary: head_dim <= 4096, heads <= 65536";
+  if ((int64_t)a.tokens * a.head_dim * ((int64_t)a.heads_q + a.heads_k) >= (int64_t(1) << 38)) return "rotary: more than 2^38 elements in a sequence";
+  if (!std::isfinite(a.amplitude)) return "rotary: amplitude must be finite";
+  if (a.batch == 0 || a.tokens == 0) return nullptr;  // nothing to do: empty tensors have no pointers
+  if (!a.q || !a.q_out || !a.inv_freq || (a.heads_k && (!a.k || !a.k_out))) return "rotary: null pointer";
+  const uintptr_t eb = (uintptr_t)elt_bytes(a.dtype);
+  if (!aligned(a.q, eb) || !aligned(a.q_out, eb) || (a.heads_k && (!aligned(a.k, eb) || !aligned(a.k_out, eb)))) return "rotary: pointer not aligned to its elements";
+  if (!aligned(a.inv_freq, 8) || (a.positions && !aligned(a.positions, 8))) return "rotary: inv_freq / positions not aligned to 8 bytes";
+  const int64_t eq[3] = {a.batch, a.tokens, a.heads_q}, ek[3] = {a.batch, a.tokens, a.heads_k};
+  if (!strides_ok(a.q_stride, eq, false) || !strides_ok(a.q_out_stride, eq, true) ||
+      (a.heads_k && (!strides_ok(a.k_stride, ek, false) || !strides_ok(a.k_out_stride, ek, true))))
+    return "rotary: strides must lie in [0, 2^40], an output's must not be 0";
+  if (a.position_stride < 0 || a.position_stride > (int64_t(1) << 40)) return "rotary: position_stride must lie in [0, 2^40]";
+  return nullptr;
+}
+
+const char* check_window_attention(const f5hip_window_attention_args& a) {
+  if (a.dtype < F5HIP_T_FP32 || a.dtype > F5HIP_T_BF16) return "window attention: dtype must be fp32, fp16 or bf16";
+  if (a.batch < 0 || a.q_tokens < 0 || a.kv_tokens < 0 || a.heads < 1 || a.kv_heads < 1) return "window attention: batch, tokens >= 0, heads >= 1";
+  if (a.heads % a.kv_heads) return "window attention: kv_heads must divide heads";
+  const int eb = elt_bytes(a.dtype);
+  if (a.head_dim < 1 || a.head_dim > 128 || (a.head_dim * eb) % 16) return "window attention: head_dim must be at most 128 and a whole multiple of 16 bytes";
+  if (a.sinks < 0) return "window attention: sinks must be >= 0";
+  if (a.align_end != 0 && a.align_end != 1) return "window attention: align_end must be 0 or 1";
+  if (!std::isfinite(a.scale)) return "window attention: scale must be finite";
+  constexpr int lim = 1 << 30;  // sums of two of them stay in 32 bits
+  if (a.q_tokens >= lim || a.kv_tokens >= lim || a.window_left >= lim || a.window_right >= lim || a.sinks >= lim)
+    return "window attention: tokens, window and sinks must be below 2^30";
+  if ((int64_t)a.batch * a.heads >= (1 << 24)) return "window attention: batch * heads must be below 2^24";
+  if ((int64_t)a.batch * a.heads * a.q_tokens >= (int64_t(1) << 31)) return "window attention: batch * heads * q_tokens must be below 2^31";
+  if (a.batch == 0 || a.q_tokens == 0) return nullptr;
+  if (!a.q || !a.out || (a.kv_tokens && (!a.k || !a.v))) return "window attention: null pointer";
+  if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16)) return "window attention: pointers must be aligned to 16 bytes";
+  if (!aligned(a.kv_len, 4) || !aligned(a.q_len, 4)) return "window attention: lengths must be aligned to 4 bytes";
+  const int64_t eq[3] = {a.batch, a.q_tokens, a.heads}, ek[3] = {a.batch, a.kv_tokens, a.kv_heads};
+  if (!strides_ok(a.q_stride, eq, false) || !strides_ok(a.out_stride, eq, true) || !strides_ok(a.k_stride, ek, false) || !strides_ok(a.v_stride, ek, false))
+    return "window attention: strides must lie in [0, 2^40], the output's must not be 0";
+  const int64_t (*all[4])[3] = {&a.q_stride, &a.k_stride, &a.v_stride, &a.out_stride};
+  for (auto* st : all)
+    for (int i = 0; i < 3; ++i)
+      if (((*st)[i] * eb) % 16) return "window attention: strides must be whole multiples of 16 bytes";
+  // a 64-key tile is addressed with 31-bit byte offsets from its first key
+  if (a.k_stride[1] * eb * 64 >= (int64_t(1) << 31) || a.v_stride[1] * eb * 64 >= (int64_t(1) << 31)) return "window attention: 64 key rows must span less than 2 GiB";
+  return nullptr;
+}
+
+extern "C" {
+int f5hip_rotary_frequencies(int rot_dim, double base, int scaling, double factor, int64_t original_length, double low, double high, double* inv_freq,
+                             double* amplitude) {
+  if (!inv_freq || !amplitude) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: null pointer");
+  if (rot_dim < 2 || (rot_dim & 1)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: rot_dim must be even and >= 2");
+  if (!(base > 0) || !std::isfinite(base)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: base must be positive");
+  if (scaling < F5HIP_ROPE_NONE || scaling > F5HIP_ROPE_YARN) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: unknown scaling");
+  if (scaling != F5HIP_ROPE_NONE && (!(factor > 0) || !std::isfinite(factor))) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: factor must be positive");
+  if (scaling == F5HIP_ROPE_NTK && rot_dim < 4) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: the base change needs rot_dim >= 4");
+  if (scaling == F5HIP_ROPE_YARN) {
+    if (low == 0 && high == 0) { low = 1; high = 32; }
+    if (original_length <= 0 || !(low >= 0) || !(high > low) || !std::isfinite(high) || !(factor >= 1))
+      return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: by parts needs original_length > 0, 0 <= low < high, factor >= 1");
+  }
+  const double b = scaling == F5HIP_ROPE_NTK ? base * std::pow(factor, (double)rot_dim / (rot_dim - 2)) : base;
+  for (int i = 0; i < rot_dim / 2; ++i) {
+    double f = std::pow(b, -2.0 * i / rot_dim);
+    if (scaling == F5HIP_ROPE_LINEAR) f /= factor;
+    if (scaling == F5HIP_ROPE_YARN) {
+      const double r = (double)original_length * f / 6.283185307179586476925;
+      const double g = std::fmin(1.0, std::fmax(0.0, (r - low) / (high - low)));
+      f *= g + (1.0 - g) / factor;
+    }
+    inv_freq[i] = f;
+  }
+  *amplitude = scaling == F5HIP_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+  return F5HIP_OK;
+}
+
+int f5hip_rotary(const f5hip_rotary_args* a, int device, void* stream) {
+  if (!a) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary: null argument");
+  if (const char* why = check_rotary(*a)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, why);
+  if (a->batch == 0 || a->tokens == 0) return F5HIP_OK;
+  return on_device(device, [&] { return launch_rotary(*a, (hipStream_t)stream); });
+}
+
+int64_t f5hip_window_attention_workspace(const f5hip_window_attention_args* a) {
+  const char* why = a ? check_window_attention(*a) : "window attention: null argument";
+  if (why) { f5hip_set_thread_error(F5HIP_ERR_INVALID, why); return -1; }
+  return a->batch == 0 || a->q_tokens == 0 ? 0 : window_attention_workspace(*a);
+}
+
+int f5hip_window_attention(const f5hip_window_attention_args* a, int device, void* stream) {
+  if (!a) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "window attention: null argument");
+  if (const char* why = check_window_attention(*a)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, why);
+  if (a->batch == 0 || a->q_tokens == 0) return F5HIP_OK;
+  const int64_t need = window_attention_workspace(*a);
+  if (a->workspace_bytes < need || (need && (!a->workspace || !aligned(a->workspace, 16))))
+    return f5hip_set_thread_error(F5HIP_ERR_INVALID, "window attention: workspace missing, too small or not aligned to 16 bytes");
+  return on_device(device, [&] { return launch_window_attention(*a, (hipStream_t)stream); });
+}
+}  // extern "C"

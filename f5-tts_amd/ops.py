@@ -1,0 +1,188 @@
+"""Operators with entry points of their own: rotary positions and sliding-window attention on the caller's tensors.
+
+They are what the sampler runs in its blocks after ``F5HipEngine.set_long_form`` (``engine.py``), for programs that bring their own layers:
+``[batch, tokens, heads, head_dim]`` tensors with any strides of the first three axes (columns of a fused q|k|v buffer, views of a cache), in
+fp32, fp16 or bf16, on the current stream of their device.  The reference calls ``apply_rotary_pos_emb`` and
+``F.scaled_dot_product_attention`` in these places (``src/f5_tts/model/modules.py:498-520``).  Nothing is kept between calls: outputs and
+workspaces come from torch's allocator on the calling stream, so calls can be captured into graphs and run side by side.  Inference only:
+an input that requires a gradient is refused.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import struct
+from typing import Optional, Tuple
+
+import torch
+
+from .binding import F5HipError, check, load_library
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # F5HIP_T_*
+_LAYOUTS = {"interleaved": 0, "half": 1}                          # F5HIP_ROTARY_*
+_SCALINGS = {None: 0, "none": 0, "linear": 1, "ntk": 2, "yarn": 3}  # F5HIP_ROPE_*
+_ROTARY = struct.Struct("@10if4P12qPP2q")   # f5hip_rotary_args
+_WINDOW = struct.Struct("@11if4P12q3Pq")    # f5hip_window_attention_args
+
+
+def _device(t: torch.Tensor) -> Tuple[int, int]:
+    """(device ordinal, current stream) of a GPU tensor."""
+    if not t.is_cuda:
+        raise F5HipError("the operators need tensors on a HIP device (torch device type 'cuda'); there is no CPU path")
+    return t.device.index, torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
+    n, s = t.shape, t.stride()  # an axis of one element may carry any stride
+    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+
+
+def _tensor(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
+    if not isinstance(t, torch.Tensor) or t.dim() != 4:
+        raise ValueError(f"{name}: a [batch, tokens, heads, head_dim] tensor is expected")
+    if t.dtype not in _TYPES:
+        raise ValueError(f"{name}: {t.dtype} is not one of float32, float16, bfloat16")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, the first tensor is {like.dtype} on {like.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: the operators are for inference (use torch.no_grad())")
+
+
+def _lengths(name: str, t: Optional[torch.Tensor], like: torch.Tensor) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.shape != like.shape[:1] or t.device != like.device:
+        raise ValueError(f"{name}: an int32 or int64 tensor of [batch] on {like.device} is expected")
+    return t.to(torch.int32).contiguous()
+
+
+def _pack(layout: struct.Struct, fields) -> bytes:
+    try:
+        return layout.pack(*fields)
+    except struct.error as e:  # a size or an option that does not fit its field
+        raise ValueError(f"argument out of range: {e}") from None
+
+
+def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0, original_length: int = 0,
+                       low: float = 0.0, high: float = 0.0, device=None) -> Tuple[torch.Tensor, float]:
+    """``(inv_freq, amplitude)`` for :func:`rotary`: ``rot_dim / 2`` frequencies in 64 bits (on ``device``), scaled for contexts ``factor``
+    times as long as trained — ``"linear"`` (positions interpolated), ``"ntk"`` (the base changed) or ``"yarn"`` (by parts: frequencies that turn
+    less than ``low`` (1) times over ``original_length`` positions are divided, those above ``high`` (32) kept, mixed between them)."""
+    if scaling not in _SCALINGS:
+        raise ValueError(f"scaling {scaling!r}: one of None, 'linear', 'ntk', 'yarn' is expected")
+    out, amplitude = (C.c_double * max(1, rot_dim // 2))(), C.c_double()
+    lib = load_library()
+    check(lib, None, lib.f5hip_rotary_frequencies(rot_dim, base, _SCALINGS[scaling], factor, original_length, low, high, out, C.byref(amplitude)))
+    return torch.tensor(list(out), dtype=torch.float64, device=device), amplitude.value
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *, amplitude: float = 1.0, positions: Optional[torch.Tensor] = None,
+           offset: int = 0, layout: str = "interleaved", rot_heads: Optional[int] = None, inverse: bool = False, out=None):
+    """Rotate the pairs of q's and k's columns by their positions' angles, both in one launch; returns ``(q', k')`` (``k`` may be None).
+
+    ``inv_freq``: float64 ``[R / 2]`` on the device (:func:`rotary_frequencies`); the first ``R`` columns of a head rotate, the others are
+    copied.  ``layout``: pairs are columns ``(2i, 2i + 1)`` ("interleaved") or ``(i, i + R / 2)`` ("half").  ``positions``: int64
+    ``[batch, tokens]`` or ``[tokens]``; without them token t stands at ``offset + t``.  ``rot_heads``: only the first so many heads of q and of
+    k rotate (the reference's ``pe_attn_head``).  ``inverse`` turns back (with amplitude 1 the inverse; in any case the operator's gradient).
+    ``out``: ``(q', k')`` to write to — the inputs themselves, or tensors that share no memory with them."""
+    _tensor("q", q)
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout {layout!r}: 'interleaved' or 'half' is expected")
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != q.device:
+        raise ValueError(f"inv_freq: a float64 vector on {q.device} is expected (rotary_frequencies)")
+    inv_freq = inv_freq.contiguous()
+    b, n, h, d = q.shape
+    if k is not None:
+        _tensor("k", k, q)
+        if k.shape[:2] != q.shape[:2] or k.shape[3] != d:
+            raise ValueError(f"k is {tuple(k.shape)}, q {tuple(q.shape)}: batch, tokens and head_dim must agree")
+        if k.stride(3) != 1 and d > 1:
+            k = k.contiguous() if out is None else k
+    if out is None:
+        q = q if q.stride(3) == 1 else q.contiguous()
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    else:
+        q_out, k_out = out
+        for name, x, y in (("q", q, q_out), ("k", k, k_out)):
+            if (x is None) != (y is None):
+                raise ValueError(f"out: one tensor for q and one for k is expected, None for a {name} that is None")
+            if x is None:
+                continue
+            _tensor(f"out for {name}", y, q)
+            if y.shape != x.shape:
+                raise ValueError(f"out for {name} is {tuple(y.shape)}, {name} {tuple(x.shape)}")
+            if x.stride(3) != 1 or y.stride(3) != 1:
+                raise ValueError(f"{name}: with out the last axis of input and output must be contiguous")
+    step = 0
+    if positions is not None:
+        if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int64 or positions.device != q.device or \
+                tuple(positions.shape) not in ((n,), (1, n), (b, n)):
+            raise ValueError(f"positions: int64 of [tokens] or [batch, tokens] on {q.device} is expected")
+        positions = positions.contiguous()
+        step = n if positions.dim() == 2 and positions.shape[0] > 1 else 0
+    device, stream = _device(q)
+    args = _pack(_ROTARY, (_TYPES[q.dtype], _LAYOUTS[layout], int(bool(inverse)), 2 * inv_freq.shape[0], b, n, h, 0 if k is None else k.shape[2], d,
+                           -1 if rot_heads is None else rot_heads, amplitude, q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(),
+                           0 if k is None else k_out.data_ptr(), *_strides(q), *((0, 0, 0) if k is None else _strides(k)), *_strides(q_out),
+                           *((0, 0, 0) if k is None else _strides(k_out)), inv_freq.data_ptr(), 0 if positions is None else positions.data_ptr(),
+                           step, offset))
+    lib = load_library()
+    check(lib, None, lib.f5hip_rotary(args, device, stream))
+    return q_out, k_out
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """The tensor, or a copy, with 16-byte aligned rows."""
+    e = t.element_size()
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any((s * e) % 16 for s in _strides(t)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: Tuple[int, int] = (-1, -1), sinks: int = 0,
+                     kv_len: Optional[torch.Tensor] = None, q_len: Optional[torch.Tensor] = None, align: str = "start",
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q ``[batch, q_tokens, heads, D]`` over k, v ``[batch, kv_tokens, kv_heads, D]`` through a sliding window; like q.
+
+    Query i stands at ``p = i`` (``align="start"``) or at the end of the keys, ``p = kv_len - q_len + i`` (``align="end"``: new tokens, one or
+    many, over a cache that holds theirs as its last).  With ``window = (left, right)`` it sees the keys ``p - left <= j <= p + right`` (negative:
+    no bound on that side; ``right = 0``: causal) and, of the first ``sinks`` keys, all that ``right`` allows.  A query that sees no key gives
+    zeros.  ``kv_len``, ``q_len``: valid keys and queries of each sequence; output rows behind ``q_len`` are zero, or left as they were in
+    ``out``.  ``scale``: 1 / sqrt(D) by default.  D: a multiple of 8 (fp32: 4) up to 128.  Keys and values that no query sees may hold
+    anything; tensors whose rows are not aligned to 16 bytes are copied first."""
+    _tensor("q", q)
+    _tensor("k", k, q)
+    _tensor("v", v, q)
+    b, n, h, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: batch and head_dim must agree, k and v in all axes")
+    if d == 0 or h == 0 or k.shape[2] == 0:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: heads and head_dim must be positive")
+    if align not in ("start", "end"):
+        raise ValueError(f"align {align!r}: 'start' or 'end' is expected")
+    kv_len, q_len = _lengths("kv_len", kv_len, q), _lengths("q_len", q_len, q)
+    left, right = window
+    if out is None:
+        out = (torch.empty if q_len is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _tensor("out", out, q)
+        if out.shape != q.shape:
+            raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
+        if out.stride(3) != 1:
+            raise ValueError("out: the last axis must be contiguous")
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    device, stream = _device(q)
+    lib = load_library()
+    fields = [_TYPES[q.dtype], b, n, k.shape[1], h, k.shape[2], d, left, right, sinks, int(align == "end"), d ** -0.5 if scale is None else scale,
+              q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *_strides(q), *_strides(k), *_strides(v), *_strides(out),
+              0 if kv_len is None else kv_len.data_ptr(), 0 if q_len is None else q_len.data_ptr(), 0, 0]
+    args = _pack(_WINDOW, fields)
+    need = lib.f5hip_window_attention_workspace(args)
+    if need < 0:
+        check(lib, None, 1)
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        fields[-2:] = [work.data_ptr(), need]
+        args = _pack(_WINDOW, fields)
+    check(lib, None, lib.f5hip_window_attention(args, device, stream))
+    return out

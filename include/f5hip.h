@@ -280,6 +280,74 @@ int f5hip_kernel_stat(const f5hip_ctx* ctx, int index, const char** name, int64_
                       double* flops, double* bytes);
 int f5hip_reset_kernel_stats(f5hip_ctx* ctx);
 
+/* ---- operators ------------------------------------------------------------------------------------ */
+/* Rotary positions and sliding-window attention as calls of their own, on the caller's tensors: what f5hip_sample runs between the q|k|v
+ * projection and the output projection of a block after f5hip_set_long_form, and what a program with its own layers calls next to it.  No
+ * context: every buffer, the workspace included, is the caller's, nothing is kept from one call for the next, and calls from any number of
+ * threads, streams and captured graphs are independent as long as their buffers are.  `device` is the HIP device ordinal the pointers
+ * belong to; the calling thread's current device is restored.  Errors: f5hip_last_error(NULL), per thread.
+ * Tensors are [batch, tokens, heads, head_dim] with any strides of the first three axes (in elements; 0 = broadcast, inputs only), the
+ * last axis contiguous. */
+enum { F5HIP_T_FP32 = 0, F5HIP_T_FP16 = 1, F5HIP_T_BF16 = 2 };
+enum { F5HIP_ROTARY_INTERLEAVED = 0 /* pairs (2i, 2i + 1) */, F5HIP_ROTARY_HALF = 1 /* pairs (i, i + rot_dim / 2) */ };
+enum { F5HIP_ROPE_NONE = 0, F5HIP_ROPE_LINEAR = 1, F5HIP_ROPE_NTK = 2, F5HIP_ROPE_YARN = 3 };
+
+/* The frequencies f_i = base^(-2i / rot_dim), i < rot_dim / 2, in 64 bits (HOST array) for contexts `factor` times as long as trained:
+ *   NONE    as they are            LINEAR  f / factor                 NTK  base * factor^(rot_dim / (rot_dim - 2)) as the base
+ *   YARN    by parts: with r = original_length f / 2 pi turns over the trained length and g = clamp((r - low) / (high - low), 0, 1),
+ *           f (g + (1 - g) / factor); *amplitude = 0.1 ln(factor) + 1 (1 for the others).  low, high: 1 and 32 where both are 0.
+ * x_transformers' RotaryEmbedding, which the reference's backbones use (model/backbones/dit.py:207,352), has the first three
+ * (interpolation_factor, base_rescale_factor). */
+int f5hip_rotary_frequencies(int rot_dim, double base, int scaling, double factor, int64_t original_length, double low, double high,
+                             double* inv_freq, double* amplitude);
+
+/* replaces: apply_rotary_pos_emb on q and k (reference model/modules.py:498-509), whatever the layout of the pairs.
+ * Token t of sequence b stands at p = positions[b * position_stride + t] (device int64; position_stride 0: one row for all sequences), or at
+ * p = first + t where positions is NULL.  The pair (x, y) of frequency i becomes amplitude (x cos - y sin, x sin + y cos) of the angle
+ * p inv_freq[i] (inverse != 0: minus the angle; the gradient of the operator).  The angle and its reduction are taken in 64 bits — exact to
+ * fp32 rounding for |p| up to 2^31 and beyond —, the rotation in fp32, and each output is rounded once.  Columns >= rot_dim and, where rot_heads >= 0,
+ * heads >= rot_heads (of q and of k: the reference's pe_attn_head, modules.py:504-509) are copied.
+ * An output may be its input (same pointer, same strides); any other overlap is not allowed.  heads_k = 0: q alone. */
+typedef struct f5hip_rotary_args {
+  int32_t dtype, layout, inverse, rot_dim;
+  int32_t batch, tokens, heads_q, heads_k, head_dim, rot_heads;
+  float amplitude;
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3]; /* batch, token, head */
+  const double* inv_freq;                                             /* device [rot_dim / 2] */
+  const int64_t* positions;
+  int64_t position_stride, first;
+} f5hip_rotary_args;
+int f5hip_rotary(const f5hip_rotary_args* args, int device, void* stream);
+
+/* replaces: F.scaled_dot_product_attention(q, k, v) (reference model/modules.py:511-520) where a query attends to a window around its own
+ * position and to the first keys of the sequence.  Query i of sequence b stands at p = i (align_end 0) or at p = kv_len[b] - q_len[b] + i
+ * (align_end 1: new tokens at the end of a cache, single ones included).  It sees key j, 0 <= j < kv_len[b], if
+ *     (window_right < 0 or j <= p + window_right)  and  (window_left < 0 or j >= p - window_left or j < sinks)
+ * (negative: no bound; window_right = 0: causal; the sinks are exempt from the left bound only).  out = softmax(scale q . k) v over the
+ * keys seen; a query that sees none gives zeros.  Query head h reads key head h / (heads / kv_heads).  Scores, softmax statistics and sums
+ * are fp32; with 16-bit types the weights are rounded to that type for the product with v (the softmax sum is that of the rounded weights).
+ *   kv_len, q_len   device int32 [batch] or NULL (kv_tokens / q_tokens), clamped into [0, kv_tokens] / [0, q_tokens].  Output rows
+ *                   i >= q_len[b] are left as they were.  Keys at and past kv_len[b] and keys in front of every query's window are not
+ *                   read, whatever they hold; a v row that SOME query of the call sees has to be finite for the others' sake.
+ *   alignment       pointers of 16 bytes, strides and head_dim whole multiples of 16 bytes; head_dim <= 128
+ *   workspace       f5hip_window_attention_workspace() bytes (may be 0) of device memory, 16-byte aligned, this call's until it ends */
+typedef struct f5hip_window_attention_args {
+  int32_t dtype, batch, q_tokens, kv_tokens, heads, kv_heads, head_dim;
+  int32_t window_left, window_right, sinks, align_end;
+  float scale;
+  const void *q, *k, *v;
+  void* out;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* batch, token, head */
+  const int32_t *kv_len, *q_len;
+  void* workspace;
+  int64_t workspace_bytes;
+} f5hip_window_attention_args;
+/* the workspace this call needs (it depends on the sizes, never on the lengths on the device), or -1: bad arguments (f5hip_last_error(NULL)) */
+int64_t f5hip_window_attention_workspace(const f5hip_window_attention_args* args);
+int f5hip_window_attention(const f5hip_window_attention_args* args, int device, void* stream);
+
 /* (The kernel microbenchmarks and fault reproducers — f5hip_bench_* — are not part of the product: include/f5hip_bench.h,
  * libf5hip_bench.so.) */
 

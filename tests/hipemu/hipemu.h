@@ -384,6 +384,15 @@ inline float shfl_xor(float v, int mask, int) {
   return r;
 }
 
+inline float shfl(float v, int src, int) {
+  WaveCtx& w = wv();
+  w.sh[blk->cur->lane] = v;
+  barrier_wait(w.bar);
+  const float r = w.sh[src & 63];
+  barrier_wait(w.bar);
+  return r;
+}
+
 // wave vote: does any lane of the wave hold a non-zero predicate?  (the kernels use it through f5_wave_any, common.h)
 inline bool wave_any(bool pred) {
   WaveCtx& w = wv();
@@ -571,6 +580,7 @@ inline void launch(dim3 grid, dim3 block, size_t lds_bytes, const std::function<
 #define gridDim hipemu::g_dim
 #define __syncthreads() hipemu::barrier_wait(hipemu::blk->bar)
 #define __shfl_xor(v, m, ...) hipemu::shfl_xor((v), (m), 64)
+#define __shfl(v, l, ...) hipemu::shfl((v), (l), 64)
 #define __amdgpu_buffer_rsrc_t hipemu::Rsrc
 #define __builtin_amdgcn_make_buffer_rsrc hipemu::make_rsrc
 #define __builtin_amdgcn_raw_buffer_load_b128 hipemu::raw_buffer_load_b128

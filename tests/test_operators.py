@@ -1,0 +1,181 @@
+"""CPU tests of the operators with entry points of their own (f5-tts_amd/ops.py): frequencies, every refusal, and the kernels' own source on the
+host shim (tests/hipemu) against the 64-bit restatement in tests/operators_oracle.py."""
+import ctypes as C
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+sys.path.insert(0, os.path.join(ROOT, "tests"))
+import operators_oracle as O  # noqa: E402
+from f5_tts_amd import binding, ops  # noqa: E402
+from test_hipemu import CLANG, engine_emu_lib  # noqa: E402,F401
+
+shim = pytest.mark.skipif(not os.path.exists(CLANG), reason="needs the ROCm host clang++")
+
+
+@pytest.fixture()
+def host(engine_emu_lib, monkeypatch):  # noqa: F811
+    """ops over the emulated library: CPU tensors are its device tensors."""
+    monkeypatch.setattr(ops, "load_library", lambda *a, **k: engine_emu_lib)
+    monkeypatch.setattr(ops, "_device", lambda t: (0, 0))
+    return ops
+
+
+def same(t):
+    return t
+
+
+# ---- frequencies -----------------------------------------------------------------------------------------------------------------------
+def test_frequencies_by_their_formulas():
+    # pow in 64 bits is within a few units of 2^-53 on either side
+    for rot in (2, 64, 96, 128):
+        f, a = ops.rotary_frequencies(rot)
+        assert a == 1.0 and f.dtype == torch.float64
+        assert torch.allclose(f, O.frequencies(rot), rtol=2.0 ** -48, atol=0)
+    f0 = O.frequencies(64)
+    f, a = ops.rotary_frequencies(64, scaling="linear", factor=4.0)
+    assert a == 1.0 and torch.allclose(f, f0 / 4, rtol=2.0 ** -48, atol=0)
+    f, a = ops.rotary_frequencies(64, scaling="ntk", factor=2.0)
+    assert a == 1.0 and torch.allclose(f, f0 * 2.0 ** (-2.0 * torch.arange(32, dtype=torch.float64) / 62), rtol=2.0 ** -47, atol=0)
+    assert f[0] == 1.0  # the fastest frequency stays, the slowest is divided by the factor
+    assert math.isclose(f[-1] * 2.0, f0[-1], rel_tol=2.0 ** -47)
+    f, a = ops.rotary_frequencies(64, scaling="yarn", factor=8.0, original_length=2048)
+    turns = 2048 * f0 / (2 * math.pi)
+    assert math.isclose(a, 0.1 * math.log(8.0) + 1)
+    assert torch.allclose(f[turns > 32], f0[turns > 32], rtol=2.0 ** -48) and torch.allclose(f[turns < 1], f0[turns < 1] / 8, rtol=2.0 ** -48)
+    between = (turns > 1) & (turns < 32)
+    assert between.any() and (f[between] < f0[between]).all() and (f[between] > f0[between] / 8).all()
+
+
+@pytest.mark.parametrize("kw", [dict(rot_dim=3), dict(rot_dim=0), dict(rot_dim=-2), dict(rot_dim=64, base=0.0), dict(rot_dim=64, base=float("nan")),
+                                dict(rot_dim=64, scaling="cubic"), dict(rot_dim=64, scaling="linear", factor=0.0), dict(rot_dim=2, scaling="ntk", factor=2.0),
+                                dict(rot_dim=64, scaling="yarn", factor=2.0), dict(rot_dim=64, scaling="yarn", factor=0.5, original_length=10),
+                                dict(rot_dim=64, scaling="yarn", factor=2.0, original_length=10, low=4.0, high=2.0)])
+def test_frequencies_refuse(kw):
+    with pytest.raises(ValueError):
+        ops.rotary_frequencies(**kw)
+
+
+# ---- refusals: before anything is launched ------------------------------------------------------------------------------------------------
+def q4(*shape, dtype=torch.float16):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_rotary_refuses(host):
+    f = O.frequencies(64)
+    q, k = q4(1, 4, 2, 64), q4(1, 4, 1, 64)
+    host.rotary(q, k, f)
+    for bad in (dict(q=q[0]), dict(q=q.long()), dict(k=k.float()), dict(k=q4(1, 5, 1, 64)), dict(k=q4(1, 4, 1, 32)), dict(f=f.float()), dict(f=f[None]),
+                dict(f=O.frequencies(128)), dict(f=f[:0]), dict(layout="both"), dict(positions=torch.zeros(4)), dict(positions=torch.zeros(5, dtype=torch.int64)),
+                dict(positions=torch.zeros(2, 4, dtype=torch.int64)), dict(rot_heads=-2), dict(amplitude=float("inf")), dict(offset=1 << 63),
+                dict(out=(q, None)), dict(out=(q, q)), dict(out=(q4(1, 4, 64, 2).transpose(2, 3), k)),
+                dict(q=q.expand(3, 4, 2, 64), k=None, out=(q.expand(3, 4, 2, 64), None)), dict(q=q.clone().float().requires_grad_(), k=None)):
+        a = dict(q=q, k=k, f=f)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            host.rotary(a.pop("q"), a.pop("k"), a.pop("f"), **a)
+    with torch.no_grad():
+        host.rotary(q.float().requires_grad_(), None, f)
+
+
+def test_window_attention_refuses(host):
+    q, k, v = q4(2, 3, 4, 64), q4(2, 5, 2, 64), q4(2, 5, 2, 64)
+    host.window_attention(q, k, v)
+    for bad in (dict(q=q[0]), dict(q=q.double()), dict(k=k.bfloat16()), dict(v=q4(2, 4, 2, 64)), dict(k=q4(1, 5, 2, 64), v=q4(1, 5, 2, 64)),
+                dict(k=q4(2, 5, 3, 64), v=q4(2, 5, 3, 64)), dict(q=q4(2, 3, 4, 60), k=q4(2, 5, 2, 60), v=q4(2, 5, 2, 60)),
+                dict(q=q4(2, 3, 4, 136), k=q4(2, 5, 2, 136), v=q4(2, 5, 2, 136)), dict(sinks=-1), dict(sinks=1 << 30), dict(window=(1 << 30, 0)),
+                dict(window=(1 << 40, 0)), dict(align="middle"), dict(scale=float("nan")), dict(kv_len=torch.zeros(3, dtype=torch.int32)),
+                dict(kv_len=torch.zeros(2)), dict(q_len=[1, 2]), dict(out=q4(2, 3, 4, 32)), dict(out=q4(2, 3, 4, 64, dtype=torch.float32)),
+                dict(out=q4(2, 3, 4, 66)[..., 1:65]), dict(out=q4(1, 3, 4, 64).expand(2, 3, 4, 64)), dict(q=q4(2, 3, 0, 64)),
+                dict(q=q4(2, 3, 4, 0), k=q4(2, 5, 2, 0), v=q4(2, 5, 2, 0)), dict(q=q.float().requires_grad_(), k=k.float(), v=v.float())):
+        a = dict(q=q, k=k, v=v)
+        a.update(bad)
+        with pytest.raises(ValueError):
+            host.window_attention(a.pop("q"), a.pop("k"), a.pop("v"), **a)
+
+
+def test_c_entries_refuse_null_and_say_why():
+    lib = binding.load_library()
+    assert lib.f5hip_rotary(None, 0, None) == 1 and b"null" in lib.f5hip_last_error(None)
+    assert lib.f5hip_window_attention(None, 0, None) == 1 and b"null" in lib.f5hip_last_error(None)
+    assert lib.f5hip_window_attention_workspace(None) == -1
+    a = C.c_double()
+    assert lib.f5hip_rotary_frequencies(64, 1e4, 0, 1.0, 0, 0.0, 0.0, None, C.byref(a)) == 1
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="only meaningful without a GPU")
+def test_no_cpu_path():
+    with pytest.raises(binding.F5HipError):
+        ops.rotary(q4(1, 1, 1, 64), None, O.frequencies(64))
+    with pytest.raises(binding.F5HipError):
+        ops.window_attention(q4(1, 1, 1, 64), q4(1, 1, 1, 64), q4(1, 1, 1, 64))
+
+
+def test_empty_calls(host):
+    f = O.frequencies(64)
+    for shape in ((0, 4, 2, 64), (2, 0, 2, 64)):
+        a, b = host.rotary(q4(*shape), q4(*shape), f)
+        assert a.shape == b.shape == shape
+        assert host.window_attention(q4(*shape), q4(shape[0], 5, 2, 64), q4(shape[0], 5, 2, 64)).shape == shape
+
+
+# ---- the kernels' source on the host shim ---------------------------------------------------------------------------------------------------
+@shim
+@pytest.mark.parametrize("name", sorted(O.ROTARY))
+def test_rotary_on_the_shim(host, name):
+    O.check_rotary(host, same, O.ROTARY[name])
+
+
+@shim
+def test_rotary_amplitude_positions_views_and_in_place_on_the_shim(host):
+    g = torch.Generator().manual_seed(1)
+    fused = torch.randn(2, 7, 6, 64, generator=g).half()
+    q, k, f = fused[:, :, :3], fused[:, :, 3:5], O.frequencies(48)
+    at = torch.randint(-1000, 200000, (2, 7), generator=g)
+    want = [O.rotary(x, f, at, amplitude=1.2, half=True) for x in (q, k)]
+    got = host.rotary(q, k, f, amplitude=1.2, positions=at, layout="half")
+    for y, (ref, tol) in zip(got, want):
+        assert O.over(y, ref, tol) <= 1
+    before = fused.clone()
+    host.rotary(q, k, f, amplitude=1.2, positions=at, layout="half", out=(q, k))  # in place, in the fused buffer
+    assert torch.equal(q, got[0]) and torch.equal(k, got[1]) and torch.equal(fused[:, :, 5:], before[:, :, 5:])
+    shared = host.rotary(before[:, :, :3], None, f, positions=at[0])[0]  # one row of positions for all sequences
+    assert torch.equal(shared, host.rotary(before[:, :, :3], None, f, positions=at[:1].expand(2, 7))[0])
+    odd = torch.randn(2 * 3 * 2 * 64 + 1, generator=g).half()[1:].view(2, 3, 2, 64)  # not aligned to more than an element
+    ref, tol = O.rotary(odd, f, torch.arange(3))
+    assert O.over(host.rotary(odd, None, f)[0], ref, tol) <= 1
+    turned = host.rotary(before[:, :, :1].expand(2, 7, 3, 64), None, f)[0]  # a broadcast input
+    assert torch.equal(turned[:, :, 0], turned[:, :, 2])
+
+
+@shim
+@pytest.mark.parametrize("name", sorted(O.ATTENTION))
+def test_window_attention_on_the_shim(host, name):
+    O.check_attention(host, same, O.ATTENTION[name])
+
+
+@shim
+def test_window_attention_ignores_what_nobody_sees_on_the_shim(host):
+    check_unseen(host, same)
+
+
+def check_unseen(ops_, to):
+    """Keys and values behind the last key, and in front of every window but no sink, may hold NaN and infinities."""
+    for name in ("token_grouped", "chunk", "token_fp32", "ragged"):
+        case = O.ATTENTION[name]
+        q, k, v, kw = O.attention_inputs(case)
+        tq, tk = q.shape[1], k.shape[1]
+        for i in range(q.shape[0]):
+            n = tk if kw["kv_len"] is None else int(kw["kv_len"][i])
+            k[i, n:], v[i, n:] = math.nan, math.inf
+            if kw["align"] == "end":
+                low = max(0, n - tq - kw["window"][0])
+                k[i, kw["sinks"]:low], v[i, kw["sinks"]:low] = math.inf, math.nan
+        ref, tol, rows = O.attention(q, k, v, **kw)
+        out = ops_.window_attention(to(q), to(k), to(v), **{x: to(y) if isinstance(y, torch.Tensor) else y for x, y in kw.items()})
+        assert O.over(out, ref, tol) <= 1
