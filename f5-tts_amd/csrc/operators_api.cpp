@@ -87,8 +87,9 @@ const char* check_window_attention(const f5hip_window_attention_args& a) {
   constexpr int lim = 1 << 30;  // sums of two of them stay in 32 bits
   if (a.q_tokens >= lim || a.kv_tokens >= lim || a.window_left >= lim || a.window_right >= lim || a.sinks >= lim)
     return "window attention: tokens, window and sinks must be below 2^30";
-  if ((int64_t)a.batch * a.heads >= (1 << 24)) return "window attention: batch * heads must be below 2^24";
-  if ((int64_t)a.batch * a.heads * a.q_tokens >= (int64_t(1) << 31)) return "window attention: batch * heads * q_tokens must be below 2^31";
+  // the grid's threads stay below 2^32
+  if ((int64_t)a.batch * a.heads >= (1 << 22)) return "window attention: batch * heads must be below 2^22";
+  if ((int64_t)a.batch * a.heads * a.q_tokens >= lim) return "window attention: batch * heads * q_tokens must be below 2^30";
   if (a.batch == 0 || a.q_tokens == 0) return nullptr;
   if (!a.q || !a.out || (a.kv_tokens && (!a.k || !a.v))) return "window attention: null pointer";
   if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16)) return "window attention: pointers must be aligned to 16 bytes";

@@ -4,25 +4,66 @@
 #include "window_attention_kernel.h"
 
 namespace {
-WindowArgs args_of(const f5hip_window_attention_args& a) {
+// Few rows (window_few_kernel: waves along the keys) up to 32 rows of a key head, many (window_rows_kernel: waves along the rows) above.  The keys are cut
+// into ranges where the row blocks alone leave CUs idle; both kernels then leave partial results that window_join_kernel merges.
+struct Plan {
+  bool few;
+  int nblk, nsplit;
+};
+Plan plan_of(const f5hip_window_attention_args& a) {
+  const int64_t rows = (int64_t)a.q_tokens * (a.heads / a.kv_heads), heads = (int64_t)a.batch * a.kv_heads;
+  Plan p;
+  p.few = rows <= 32;
+  const int per = p.few ? 32 : 128;
+  p.nblk = (int)((rows + per - 1) / per);
+  // the most keys a row block can see
+  const int64_t tokens = std::min<int64_t>(a.q_tokens, per / (a.heads / a.kv_heads) + 2);
+  int64_t keys = a.kv_tokens;
+  if (a.window_left >= 0 && a.window_right >= 0) keys = std::min<int64_t>(keys, (int64_t)a.window_left + a.window_right + tokens + std::min(a.sinks, a.kv_tokens));
+  const int64_t blocks = heads * p.nblk, want = (512 + blocks - 1) / blocks, most = p.few ? keys / 512 : keys / 256;
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, most), 64));
+  return p;
+}
+int64_t parts(const f5hip_window_attention_args& a, const Plan& p) { return (int64_t)a.batch * a.heads * a.q_tokens * p.nsplit; }
+
+template <typename T>
+hipError_t launch(const WindowArgs& w, const Plan& p, hipStream_t s) {
+  const auto go = [&](auto DP) {
+    constexpr int dp = decltype(DP)::value;
+    if (p.few) hipLaunchKernelGGL((window_few_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(64 * FEW_WAVES), 0, s, w);
+    else hipLaunchKernelGGL((window_rows_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
+  };
+  if (w.dim <= 64) go(std::integral_constant<int, 64>{});
+  else if (w.dim <= 96) go(std::integral_constant<int, 96>{});
+  else go(std::integral_constant<int, 128>{});
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || w.nsplit == 1) return e;
+  const int64_t threads = (int64_t)w.batch * w.heads * w.tq * (w.dim / 4);
+  hipLaunchKernelGGL((window_join_kernel<T>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, w);
+  return hipGetLastError();
+}
+}  // namespace
+
+int64_t window_attention_workspace(const f5hip_window_attention_args& a) {
+  const Plan p = plan_of(a);
+  return p.nsplit == 1 ? 0 : parts(a, p) * (a.head_dim + 2) * 4;
+}
+
+hipError_t launch_window_attention(const f5hip_window_attention_args& a, hipStream_t s) {
+  const Plan p = plan_of(a);
   WindowArgs w{};
   w.q = a.q; w.k = a.k; w.v = a.v; w.out = a.out;
   for (int i = 0; i < 3; ++i) { w.q_stride[i] = a.q_stride[i]; w.k_stride[i] = a.k_stride[i]; w.v_stride[i] = a.v_stride[i]; w.out_stride[i] = a.out_stride[i]; }
   w.kv_len = a.kv_len; w.q_len = a.q_len;
   w.batch = a.batch; w.tq = a.q_tokens; w.tk = a.kv_tokens; w.heads = a.heads; w.kv_heads = a.kv_heads; w.group = a.heads / a.kv_heads; w.dim = a.head_dim;
   w.left = a.window_left; w.right = a.window_right; w.sinks = a.sinks; w.align_end = a.align_end;
-  w.scale_log2 = a.scale * 1.4426950408889634f;
-  return w;
-}
-}  // namespace
-
-int64_t window_attention_workspace(const f5hip_window_attention_args&) { return 0; }
-
-hipError_t launch_window_attention(const f5hip_window_attention_args& a, hipStream_t s) {
-  const WindowArgs w = args_of(a);
-  const dim3 grid((unsigned)((int64_t)a.q_tokens * a.batch * a.heads));
-  if (a.dtype == F5HIP_T_FP16) hipLaunchKernelGGL((window_attention_simple_kernel<f16>), grid, dim3(64), 0, s, w);
-  else if (a.dtype == F5HIP_T_BF16) hipLaunchKernelGGL((window_attention_simple_kernel<bf16>), grid, dim3(64), 0, s, w);
-  else hipLaunchKernelGGL((window_attention_simple_kernel<float>), grid, dim3(64), 0, s, w);
-  return hipGetLastError();
+  w.scale_log2 = std::max(std::fabs(a.scale) * 1.4426950408889634f, 1e-30f);  // (0 would turn a masked score into NaN)
+  w.negate = a.scale < 0 ? (a.dtype == F5HIP_T_FP32 ? 0x80000000u : 0x80008000u) : 0u;
+  w.nblk = p.nblk; w.nsplit = p.nsplit;
+  w.nwg = (int)((int64_t)a.batch * a.kv_heads * p.nblk * p.nsplit);
+  w.part_o = static_cast<float*>(a.workspace);
+  w.part_ml = w.part_o ? w.part_o + parts(a, p) * a.head_dim : nullptr;
+  if (a.dtype == F5HIP_T_FP16) return launch<f16>(w, p, s);
+  if (a.dtype == F5HIP_T_BF16) return launch<bf16>(w, p, s);
+  return launch<float>(w, p, s);
 }

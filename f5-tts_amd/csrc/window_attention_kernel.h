@@ -1,5 +1,18 @@
-// window_attention_kernel.h — sliding-window attention with sinks (include/f5hip.h f5hip_window_attention); the launch rules are in
-// window_attention.hip.
+// window_attention_kernel.h — sliding-window attention with sinks (include/f5hip.h f5hip_window_attention).  A header so that tests/hipemu can
+// compile the same source for the host; the launch rules are in window_attention.hip.
+//
+// Rows.  The query heads that share a key head are rows of one matrix: row R of (sequence, key head) is token R / group, head R % group, so
+// a key tile is read once for all of them, and one new token of a model with grouped heads already fills part of a 32-row tile.
+// Keys.  A block of rows visits [0, sinks) and the union of its rows' windows, [low, high) — or [0, high) where the two meet — in tiles that
+// start at 0 and at `low`: whatever lies between, or past the last key, is not read (rows behind a tile's last key come from the buffer
+// descriptor's bounds check as zeros).  Only tiles on a border of some row's window take the mask.
+// Product.  S^T = K Q^T on 32x32 matrix instructions leaves a lane 16 keys of ONE query row, so maxima and sums are register work and one
+// half-wave exchange; those registers are, as they stand, the other operand of O^T += V^T P^T (the contraction runs over keys in the
+// accumulator's own order), so P never moves.  V^T fragments come from row-major V tiles by the transposing LDS read (16-bit types) or as
+// single floats.
+// Softmax.  exp2(c s - c m) with c = scale log2 e > 0 (a negative scale's sign is folded into q).  m is a reference, not the exact maximum: it
+// is raised (and O, l rescaled) only where a tile exceeds it by more than 8 in the exponent.  fp16 weights are held times 2^7, up to 2^15: those
+// as small as 2^-21 of the row's largest are then normal numbers, rounded relative to themselves.
 #pragma once
 #include <math.h>
 
@@ -14,47 +27,498 @@ struct WindowArgs {
   const int32_t *kv_len, *q_len;
   int batch, tq, tk, heads, kv_heads, group, dim;
   int left, right, sinks, align_end;
-  float scale_log2;  // scale * log2(e)
+  float scale_log2;       // |scale| log2(e), > 0
+  uint32_t negate;        // sign bits to flip in q (a negative scale)
+  int nblk, nsplit, nwg;  // row blocks of a (sequence, key head), key ranges of a row block, workgroups
+  float *part_o, *part_ml;  // nsplit > 1: [rows, nsplit, dim] unnormalised, [rows, nsplit, 2] (c m - BIAS, l); rows = (sequence, head, token)
 };
 
-// One wave per query row: 64 keys at a time, a lane per key for the scores, a lane per column for the product with v.
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
 template <typename T>
-__global__ __launch_bounds__(64) void window_attention_simple_kernel(WindowArgs a) {
-  const int lane = threadIdx.x, bh = blockIdx.x / a.tq, i = blockIdx.x - bh * a.tq, b = bh / a.heads, head = bh - b * a.heads;
-  const int n = a.kv_len ? min(max(a.kv_len[b], 0), a.tk) : a.tk, nq = a.q_len ? min(max(a.q_len[b], 0), a.tq) : a.tq;
-  if (i >= nq) return;
-  const int p = a.align_end ? n - nq + i : i;
-  const int end = a.right < 0 ? n : max(0, min(n, p + a.right + 1)), begin = a.left < 0 ? 0 : min(max(0, p - a.left), end);
-  const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + i * a.q_stride[1] + head * a.q_stride[2];
-  const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + (head / a.group) * a.k_stride[2];
-  const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + (head / a.group) * a.v_stride[2];
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  const auto keys = [&](int from, int to) {
-    for (int j0 = from; j0 < to; j0 += 64) {
-      float s = -INFINITY;
-      if (j0 + lane < to) {
-        s = 0.f;
-        for (int d = 0; d < a.dim; ++d) s = fmaf((float)q[d], (float)k[(int64_t)(j0 + lane) * a.k_stride[1] + d], s);
-        s *= a.scale_log2;
-      }
-      const float mn = fmaxf(m, wave_max(s)), al = exp2f(m - mn), w = exp2f(s - mn);
+struct Win;  // what differs between the element types
+template <>
+struct Win<f16> {
+  static constexpr int KT = 64;
+  static constexpr float BIAS = 7.0f;
+  static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const f16x2 v = {(f16)x, (f16)y};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  static __device__ __forceinline__ float add2(uint32_t p, float acc) { return f5_sum2_f16(p, acc); }
+};
+template <>
+struct Win<bf16> {
+  static constexpr int KT = 64;
+  static constexpr float BIAS = 0.0f;
+  static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const bf16x2 v = {(bf16)x, (bf16)y};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  static __device__ __forceinline__ float add2(uint32_t p, float acc) {
+    return acc + (__builtin_bit_cast(float, p << 16) + __builtin_bit_cast(float, p & 0xffff0000u));
+  }
+};
+template <>
+struct Win<float> {
+  static constexpr int KT = 32;
+  static constexpr float BIAS = 0.0f;
+  static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
+    Frag x, y;
+    x.u = a;
+    y.u = b;
+    Mma32<float>::mma(c, x, y);
+  }
+};
+
+// 4 rows of a row-major 16-bit tile, transposed: lanes 4 r + c of a group of 16 name 4 columns (8 bytes) of row r, lane i gets column i of the
+// four rows (ds_read_b64_tr_b16)
+__device__ __forceinline__ uint2 lds_read_transposed(const char* p) {
+#ifdef F5_HIPEMU
+  return hipemu::ds_read_tr16(p);
+#else
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+#endif
+}
+
+// max over the lane and its partner in the other half-wave (the same query row)
+__device__ __forceinline__ float both_halves_max(float x) {
+  uint32_t a = __builtin_bit_cast(uint32_t, x), b = a;
+  f5_swap32(a, b);
+  return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float both_halves_sum(float x) {
+  uint32_t a = __builtin_bit_cast(uint32_t, x), b = a;
+  f5_swap32(a, b);
+  return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+// the windows of tokens: [low(p), high(p)) and, of the sinks, [0, min(sinks, high(p)))
+struct Span {
+  int n, left, right;
+  __device__ __forceinline__ int high(int p) const { return right < 0 ? n : max(0, min(n, p + right + 1)); }
+  __device__ __forceinline__ int low(int p) const { return left < 0 ? 0 : max(0, p - left); }
+};
+
+// a tile's rows through a buffer descriptor: rows at and past `rows`, and columns past the head's, read as zeros
+__device__ __forceinline__ BufRsrc tile_rsrc(const char* base, int64_t stride_bytes, int key0, int rows, int dim_bytes) {
+  const uint32_t bytes = rows > 0 ? (uint32_t)((rows - 1) * (int)stride_bytes + dim_bytes) : 0u;
+  return make_rsrc(base + (int64_t)key0 * stride_bytes, bytes);
+}
+
+// the running softmax of one 32-row group: O^T (32 columns a block), reference maximum, row sum
+template <typename T, int DP>
+struct Rows {
+  static constexpr int EB = sizeof(T), ND = DP / 32, NKS = DP * EB / 32;
+  static constexpr int K_ROWB = DP * EB + 16;                              // 32 rows read 16 bytes each without conflicts
+  static constexpr int V_ROWB = EB == 4 ? DP * 4 + 32 : (DP == 64 ? 192 : 320);  // 16 bit: 4 rows start 64 bytes apart in the 256-byte bank row
+  f32x16 o[ND];
+  float m, mc, l;  // reference maximum (raw score; -inf: nothing seen), c m - BIAS (0 then), this lane's share of the row sum
+  int lo, hi;      // the lane's row: its window
+  uint4 fq[NKS];
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    m = -INFINITY;
+    mc = 0.f;
+    l = 0.f;
+  }
+
+  // scores of NB blocks of 32 keys -> weights: mask (where `border`), reference maximum, exponentials, row sum
+  template <int NB>
+  __device__ __forceinline__ void softmax(f32x16 (&s)[NB], int key0, int kend, int half, bool border, const WindowArgs& a) {
+    const float c = a.scale_log2;
+    if (border) {
+      const int base = key0 + 4 * half, e = min(hi, kend) - base, b = lo - base, k = a.sinks - base;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int off = n * 32 + (r & 3) + 8 * (r >> 2);
+          s[n][r] = (off < e) & ((off >= b) | (off < k)) ? s[n][r] : -INFINITY;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
+    mx = both_halves_max(mx);
+    if (f5_wave_any(fmaf(mx, c, -mc) > 8.0f + Win<T>::BIAS || (m == -INFINITY && mx > -INFINITY))) {
+      const float mn = fmaxf(m, mx), mnc = mn == -INFINITY ? 0.f : fmaf(mn, c, -Win<T>::BIAS);
+      const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - mnc);
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= al;
+      l *= al;
       m = mn;
-      l = l * al + wave_sum(w);
-      o0 *= al;
-      o1 *= al;
-      for (int t = 0; t < min(64, to - j0); ++t) {
-        const float wt = __shfl(w, t, 64);
-        const T* r = v + (int64_t)(j0 + t) * a.v_stride[1];
-        if (lane < a.dim) o0 = fmaf(wt, (float)r[lane], o0);
-        if (lane + 64 < a.dim) o1 = fmaf(wt, (float)r[lane + 64], o1);
+      mc = mnc;
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -mc));
+  }
+
+  // O^T += V^T P^T over NB blocks of 32 keys whose V rows lie at sv
+  template <int NB>
+  __device__ __forceinline__ void product(const f32x16 (&s)[NB], const char* sv, int lane) {
+    const int half = lane >> 5;
+    if constexpr (EB == 2) {
+      const char* at = sv + (4 * half + ((lane & 15) >> 2)) * V_ROWB + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#pragma unroll
+      for (int g = 0; g < 2 * NB; ++g) {  // 16 keys: the lane's are 16 g + 4 half + 0..3 and 8 on
+        uint32_t p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = Win<T>::pack(s[g >> 1][8 * (g & 1) + 2 * e], s[g >> 1][8 * (g & 1) + 2 * e + 1]);
+          l = Win<T>::add2(p[e], l);  // the sum is that of the rounded weights: numerator and denominator see the same ones
+        }
+        const uint4 fp = make_uint4(p[0], p[1], p[2], p[3]);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const uint2 v0 = lds_read_transposed(at + g * 16 * V_ROWB + d * 64), v1 = lds_read_transposed(at + (g * 16 + 8) * V_ROWB + d * 64);
+          Win<T>::mma(o[d], make_uint4(v0.x, v0.y, v1.x, v1.y), fp);
+        }
       }
+    } else {
+      const char* at = sv + 4 * half * V_ROWB + (lane & 31) * 4;
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          l += s[n][r];
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(at + (n * 32 + (r & 3) + 8 * (r >> 2)) * V_ROWB + d * 128), s[n][r], o[d], 0, 0, 0);
+        }
+    }
+  }
+};
+
+// four neighbouring columns of an output row
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float x0, float x1, float x2, float x3) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(x0, x1, x2, x3);
+  else *reinterpret_cast<uint2*>(p) = make_uint2(Win<T>::pack(x0, x1), Win<T>::pack(x2, x3));
+}
+
+// XCD-aware placement: block b runs on XCD b % 8, so give each XCD a contiguous range of the order — the row blocks and key ranges of one key head
+// are neighbours in it and share an L2.  A bijection for any grid.
+__device__ __forceinline__ int xcd_order(int b, int n) {
+  const int q = n >> 3, r = n & 7, x = b & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (b >> 3);
+}
+
+// ---- many rows: 4 waves x 32 rows, K and V tiles shared through LDS, two stages --------------------------------------------------------------
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
+  using R = Rows<T, DP>;
+  constexpr int KT = Win<T>::KT, NB = KT / 32, EB = R::EB, CPR = DP * EB / 16, NL = KT * CPR / 256;
+  constexpr int VOFF = KT * R::K_ROWB, STAGE = VOFF + KT * R::V_ROWB;
+  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, ql = lane & 31;
+  int L = xcd_order((int)blockIdx.x, a.nwg);
+  const int ks = L % a.nsplit;
+  L /= a.nsplit;
+  const int blk = L % a.nblk, bh = L / a.nblk, b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
+  const int n = a.kv_len ? max(0, min(a.kv_len[b], a.tk)) : a.tk, nq = a.q_len ? max(0, min(a.q_len[b], a.tq)) : a.tq;
+  const int first = blk * 128 / a.group;
+  if (first >= nq) return;  // (the whole workgroup: no barrier has been reached)
+  const int p0 = a.align_end ? n - nq : 0;
+  const Span sp{n, a.left, a.right};
+  const int last = min(nq - 1, (blk * 128 + 127) / a.group);
+  const int khigh = sp.high(p0 + last), klow = min(sp.low(p0 + first), khigh), ksink = min(a.sinks, khigh);
+  const int ea = klow <= ksink ? 0 : ksink, bb = klow <= ksink ? 0 : klow;  // keys [0, ea) and [bb, khigh)
+  const int na = (ea + KT - 1) / KT, nt = na + (khigh - bb + KT - 1) / KT;
+  const int t0 = (int)((int64_t)ks * nt / a.nsplit), t1 = (int)((int64_t)(ks + 1) * nt / a.nsplit);
+
+  // the wave's rows, the lane's row
+  const int row = blk * 128 + wave * 32 + ql, tok = row / a.group, g = row - tok * a.group, head = kvh * a.group + g;
+  const bool live = tok < nq;
+  const int wfirst = min(nq - 1, (blk * 128 + wave * 32) / a.group), wlast = min(nq - 1, (blk * 128 + wave * 32 + 31) / a.group);
+  const bool idle = (blk * 128 + wave * 32) / a.group >= nq;
+  const int whi0 = sp.high(p0 + wfirst), whi1 = sp.high(p0 + wlast), wlo0 = sp.low(p0 + wfirst), wlo1 = sp.low(p0 + wlast);
+  R st;
+  st.reset();
+  st.lo = sp.low(p0 + tok);
+  st.hi = live ? sp.high(p0 + tok) : 0;
+  const T* qp = static_cast<const T*>(a.q) + b * a.q_stride[0] + tok * a.q_stride[1] + head * a.q_stride[2];
+#pragma unroll
+  for (int k = 0; k < R::NKS; ++k) {
+    const int col = (k * 32 + half * 16) / EB;
+    uint4 u = live && col < a.dim ? *reinterpret_cast<const uint4*>(qp + col) : make_uint4(0, 0, 0, 0);
+    u.x ^= a.negate; u.y ^= a.negate; u.z ^= a.negate; u.w ^= a.negate;
+    st.fq[k] = u;
+  }
+
+  const char* kb = static_cast<const char*>(a.k) + (b * a.k_stride[0] + kvh * a.k_stride[2]) * EB;
+  const char* vb = static_cast<const char*>(a.v) + (b * a.v_stride[0] + kvh * a.v_stride[2]) * EB;
+  const int64_t ksb = a.k_stride[1] * EB, vsb = a.v_stride[1] * EB;
+  const int dimb = a.dim * EB;
+  uint4 rk[NL], rv[NL];
+  const auto tile = [&](int t, int& key0, int& kend) {
+    key0 = t < na ? t * KT : bb + (t - na) * KT;
+    kend = t < na ? ea : khigh;
+  };
+  const auto load = [&](int t) {
+    int key0, kend;
+    tile(t, key0, kend);
+    const int rows = min(KT, kend - key0);
+    const BufRsrc Kr = tile_rsrc(kb, ksb, key0, rows, dimb), Vr = tile_rsrc(vb, vsb, key0, rows, dimb);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
+      const bool in = col * 16 < dimb && r < rows;
+      rk[i] = buffer_load_b128(Kr, in ? (uint32_t)(r * (int)ksb + col * 16) : OOB_ROW);
+      rv[i] = buffer_load_b128(Vr, in ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW);
     }
   };
-  keys(0, min(a.sinks, begin));
-  keys(begin, end);
-  T* o = static_cast<T*>(a.out) + b * a.out_stride[0] + i * a.out_stride[1] + head * a.out_stride[2];
+  const auto store = [&](int stage) {
+    char* base = smem + stage * STAGE;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
+      *reinterpret_cast<uint4*>(base + r * R::K_ROWB + col * 16) = rk[i];
+      *reinterpret_cast<uint4*>(base + VOFF + r * R::V_ROWB + col * 16) = rv[i];
+    }
+  };
+
+  if (t0 < t1) {
+    load(t0);
+    store(0);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    if (t + 1 < t1) load(t + 1);
+    int key0, kend;
+    tile(t, key0, kend);
+    const bool unseen = key0 >= whi1 || (min(key0 + KT, kend) <= wlo0 && key0 >= a.sinks);
+    if (!idle && !unseen) {
+      const bool border = !(key0 + KT <= min(whi0, kend) && (key0 >= wlo1 || key0 + KT <= a.sinks));
+      const char* base = smem + ((t - t0) & 1) * STAGE;
+      const char* sk = base + ql * R::K_ROWB + half * 16;
+      f32x16 s[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < R::NKS; ++k) Win<T>::mma(s[nb], *reinterpret_cast<const uint4*>(sk + nb * 32 * R::K_ROWB + k * 32), st.fq[k]);
+      }
+      st.softmax(s, key0, kend, half, border, a);
+      st.product(s, base + VOFF, lane);
+    }
+    if (t + 1 < t1) store((t + 1 - t0) & 1);
+    __syncthreads();
+  }
+
+  const float l = both_halves_sum(st.l);
+  if (!live) return;
+  if (a.nsplit > 1) {
+    const int64_t part = (((int64_t)b * a.heads + head) * a.tq + tok) * a.nsplit + ks;
+    float* po = a.part_o + part * a.dim;
+#pragma unroll
+    for (int d = 0; d < R::ND; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int col = d * 32 + 8 * c + 4 * half;
+        if (col < a.dim) *reinterpret_cast<float4*>(po + col) = make_float4(st.o[d][4 * c], st.o[d][4 * c + 1], st.o[d][4 * c + 2], st.o[d][4 * c + 3]);
+      }
+    if (half == 0) {
+      a.part_ml[part * 2] = st.m == -INFINITY ? -INFINITY : st.mc;
+      a.part_ml[part * 2 + 1] = l;
+    }
+    return;
+  }
   const float inv = l > 0.f ? 1.0f / l : 0.f;
-  if (lane < a.dim) o[lane] = (T)(o0 * inv);
-  if (lane + 64 < a.dim) o[lane + 64] = (T)(o1 * inv);
+  T* op = static_cast<T*>(a.out) + b * a.out_stride[0] + tok * a.out_stride[1] + head * a.out_stride[2];
+#pragma unroll
+  for (int d = 0; d < R::ND; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int col = d * 32 + 8 * c + 4 * half;
+      if (col < a.dim) store4(op + col, st.o[d][4 * c] * inv, st.o[d][4 * c + 1] * inv, st.o[d][4 * c + 2] * inv, st.o[d][4 * c + 3] * inv);
+    }
+}
+
+// ---- few rows: one 32-row group, the waves along the keys ----------------------------------------------------------------------------------------
+// Every wave walks 32-key tiles of its own (tile t belongs to wave t % NW): K straight into operand registers, V through the wave's own LDS rows, no
+// barrier on the way, the next tile's loads in flight meanwhile; the waves' results meet in LDS at the end, in a fixed order.
+constexpr int FEW_WAVES = 8;
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * FEW_WAVES, 1) void window_few_kernel(WindowArgs a) {
+  using R = Rows<T, DP>;
+  constexpr int NW = FEW_WAVES, KT = 32, EB = R::EB, CPR = DP * EB / 16, NL = KT * CPR / 64;
+  constexpr int VB = KT * R::V_ROWB, MERGE = NW * 32 * 33 * 4;
+  __shared__ __attribute__((aligned(16))) char smem[NW * VB > MERGE ? NW * VB : MERGE];
+  __shared__ float sml[NW][32][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, ql = lane & 31;
+  int L = xcd_order((int)blockIdx.x, a.nwg);
+  const int ks = L % a.nsplit;
+  L /= a.nsplit;
+  const int blk = L % a.nblk, bh = L / a.nblk, b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
+  const int n = a.kv_len ? max(0, min(a.kv_len[b], a.tk)) : a.tk, nq = a.q_len ? max(0, min(a.q_len[b], a.tq)) : a.tq;
+  const int first = blk * 32 / a.group;
+  if (first >= nq) return;  // (the whole workgroup)
+  const int p0 = a.align_end ? n - nq : 0;
+  const Span sp{n, a.left, a.right};
+  const int last = min(nq - 1, (blk * 32 + 31) / a.group);
+  const int high0 = sp.high(p0 + first), khigh = sp.high(p0 + last), low1 = sp.low(p0 + last), klow = min(sp.low(p0 + first), khigh), ksink = min(a.sinks, khigh);
+  const int ea = klow <= ksink ? 0 : ksink, bb = klow <= ksink ? 0 : klow;
+  const int na = (ea + KT - 1) / KT, nt = na + (khigh - bb + KT - 1) / KT;
+  const int t0 = (int)((int64_t)ks * nt / a.nsplit), t1 = (int)((int64_t)(ks + 1) * nt / a.nsplit);
+
+  const int row = blk * 32 + ql, tok = row / a.group, g = row - tok * a.group, head = kvh * a.group + g;
+  const bool live = tok < nq;
+  R st;
+  st.reset();
+  st.lo = sp.low(p0 + tok);
+  st.hi = live ? sp.high(p0 + tok) : 0;
+  const T* qp = static_cast<const T*>(a.q) + b * a.q_stride[0] + tok * a.q_stride[1] + head * a.q_stride[2];
+#pragma unroll
+  for (int k = 0; k < R::NKS; ++k) {
+    const int col = (k * 32 + half * 16) / EB;
+    uint4 u = live && col < a.dim ? *reinterpret_cast<const uint4*>(qp + col) : make_uint4(0, 0, 0, 0);
+    u.x ^= a.negate; u.y ^= a.negate; u.z ^= a.negate; u.w ^= a.negate;
+    st.fq[k] = u;
+  }
+  const char* kb = static_cast<const char*>(a.k) + (b * a.k_stride[0] + kvh * a.k_stride[2]) * EB;
+  const char* vb = static_cast<const char*>(a.v) + (b * a.v_stride[0] + kvh * a.v_stride[2]) * EB;
+  const int64_t ksb = a.k_stride[1] * EB, vsb = a.v_stride[1] * EB;
+  const int dimb = a.dim * EB;
+  char* sv = smem + wave * VB;
+
+  const auto tile = [&](int t, int& key0, int& kend) {
+    key0 = t < na ? t * KT : bb + (t - na) * KT;
+    kend = t < na ? ea : khigh;
+  };
+  const auto load = [&](int t, uint4 (&fk)[R::NKS], uint4 (&rv)[NL]) {
+    int key0, kend;
+    tile(t, key0, kend);
+    const int rows = min(KT, kend - key0);
+    const BufRsrc Kr = tile_rsrc(kb, ksb, key0, rows, dimb), Vr = tile_rsrc(vb, vsb, key0, rows, dimb);
+#pragma unroll
+    for (int k = 0; k < R::NKS; ++k) {
+      const int col = k * 32 + half * 16;
+      fk[k] = buffer_load_b128(Kr, col < dimb && ql < rows ? (uint32_t)(ql * (int)ksb + col) : OOB_ROW);
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int c = lane + i * 64, r = c / CPR, col = c - r * CPR;
+      rv[i] = buffer_load_b128(Vr, col * 16 < dimb && r < rows ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW);
+    }
+  };
+  const auto process = [&](int t, const uint4 (&fk)[R::NKS], const uint4 (&rv)[NL]) {
+    int key0, kend;
+    tile(t, key0, kend);
+    f32x16 s[1];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
+#pragma unroll
+    for (int k = 0; k < R::NKS; ++k) Win<T>::mma(s[0], fk[k], st.fq[k]);
+    wave_lds_sync();  // the last tile's reads of these rows come before
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int c = lane + i * 64, r = c / CPR, col = c - r * CPR;
+      *reinterpret_cast<uint4*>(sv + r * R::V_ROWB + col * 16) = rv[i];
+    }
+    const bool border = !(key0 + KT <= min(high0, kend) && (key0 >= low1 || key0 + KT <= a.sinks));
+    st.softmax(s, key0, kend, half, border, a);
+    wave_lds_sync();
+    st.product(s, sv, lane);
+  };
+  uint4 k0[R::NKS], v0[NL], k1[R::NKS], v1[NL];
+  int t = t0 + wave;
+  if (t < t1) load(t, k0, v0);
+  while (t < t1) {
+    if (t + NW < t1) load(t + NW, k1, v1);
+    process(t, k0, v0);
+    t += NW;
+    if (t >= t1) break;
+    if (t + NW < t1) load(t + NW, k0, v0);
+    process(t, k1, v1);
+    t += NW;
+  }
+
+  // the waves' parts: common reference, then 32 columns at a time through LDS, summed in the waves' order
+  const float l = both_halves_sum(st.l);
+  if (half == 0) {
+    sml[wave][ql][0] = st.m == -INFINITY ? -INFINITY : st.mc;
+    sml[wave][ql][1] = l;
+  }
+  __syncthreads();
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) top = fmaxf(top, sml[w][ql][0]);
+  const float mine = sml[wave][ql][0], f = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - top);
+  float* sm = reinterpret_cast<float*>(smem);
+  for (int d = 0; d < R::ND; ++d) {
+    __syncthreads();  // the V rows, or the columns before, have been read
+#pragma unroll
+    for (int dd = 0; dd < R::ND; ++dd)  // (a register array is indexed with constants only)
+      if (dd == d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sm[(wave * 32 + (r & 3) + 8 * (r >> 2) + 4 * half) * 33 + ql] = st.o[dd][r] * f;
+    __syncthreads();
+    for (int v = tid; v < 1024; v += 64 * NW) {
+      const int rr = v >> 5, cc = v & 31, col = d * 32 + cc, orow = blk * 32 + rr, otok = orow / a.group;
+      if (otok >= nq || col >= a.dim) continue;
+      const int ohead = kvh * a.group + (orow - otok * a.group);
+      float x = 0.f, rtop = -INFINITY, rl = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        x += sm[(w * 32 + cc) * 33 + rr];
+        rtop = fmaxf(rtop, sml[w][rr][0]);
+      }
+#pragma unroll
+      for (int w = 0; w < NW; ++w) rl += sml[w][rr][0] == -INFINITY ? 0.f : sml[w][rr][1] * __builtin_amdgcn_exp2f(sml[w][rr][0] - rtop);
+      if (a.nsplit > 1) {
+        const int64_t part = (((int64_t)b * a.heads + ohead) * a.tq + otok) * a.nsplit + ks;
+        a.part_o[part * a.dim + col] = x;
+        if (col == 0) { a.part_ml[part * 2] = rtop; a.part_ml[part * 2 + 1] = rl; }
+      } else {
+        T* op = static_cast<T*>(a.out) + b * a.out_stride[0] + otok * a.out_stride[1] + ohead * a.out_stride[2];
+        op[col] = (T)(rl > 0.f ? x / rl : 0.f);
+      }
+    }
+  }
+}
+
+// ---- join of the key ranges: a thread per four columns of a row -----------------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
+  const int quads = a.dim / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / quads;
+  if (row >= (int64_t)a.batch * a.heads * a.tq) return;
+  const int col = (int)(id - row * quads) * 4, bh = (int)(row / a.tq), tok = (int)(row - (int64_t)bh * a.tq), b = bh / a.heads, head = bh - b * a.heads;
+  const int nq = a.q_len ? max(0, min(a.q_len[b], a.tq)) : a.tq;
+  if (tok >= nq) return;
+  const float* ml = a.part_ml + row * a.nsplit * 2;
+  const float* po = a.part_o + row * a.nsplit * a.dim + col;
+  float top = -INFINITY;
+  for (int s = 0; s < a.nsplit; ++s) top = fmaxf(top, ml[2 * s]);
+  float l = 0.f, x0 = 0.f, x1 = 0.f, x2 = 0.f, x3 = 0.f;
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float f = ml[2 * s] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[2 * s] - top);
+    const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)s * a.dim);
+    l += f * ml[2 * s + 1];
+    x0 += f * x.x; x1 += f * x.y; x2 += f * x.z; x3 += f * x.w;
+  }
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  T* op = static_cast<T*>(a.out) + b * a.out_stride[0] + tok * a.out_stride[1] + head * a.out_stride[2] + col;
+  store4(op, x0 * inv, x1 * inv, x2 * inv, x3 * inv);
 }
 }  // namespace

@@ -190,6 +190,7 @@ struct Fiber {
 struct WaveCtx {
   Barrier bar;
   float a[64][8], b[64][8], sh[64];
+  const void* ptr[64];            // ds_read_tr16
   float qa[64][32], qb[64][32];  // decoded MX operands (mfma_scale_32x32x64_fp6)
 };
 struct BlockCtx {
@@ -278,6 +279,36 @@ inline f16v mfma_32x32x16_f16(h8 a, h8 b, f16v c, int, int, int) {
   }
   barrier_wait(w.bar);
   return c;
+}
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+inline f16v mfma_32x32x16_bf16(bf8v a, bf8v b, f16v c, int, int, int) {
+  WaveCtx& w = wv();
+  const int lane = blk->cur->lane;
+  for (int e = 0; e < 8; ++e) { w.a[lane][e] = (float)a[e]; w.b[lane][e] = (float)b[e]; }
+  barrier_wait(w.bar);
+  const int j = lane & 31, hi = lane >> 5;
+  for (int r = 0; r < 16; ++r) {
+    const int i = (r & 3) + 8 * (r >> 2) + 4 * hi;
+    float s = 0.f;
+    for (int k = 0; k < 16; ++k) s += w.a[i + 32 * (k >> 3)][k & 7] * w.b[j + 32 * (k >> 3)][k & 7];
+    c[r] += s;
+  }
+  barrier_wait(w.bar);
+  return c;
+}
+// ds_read_b64_tr_b16 (lane layout checked on the GPU): in a group of 16 lanes, lane 4 r + c names 4 halves of row r (columns 4 c ..), lane i gets
+// column i of rows 0 .. 3
+inline uint2 ds_read_tr16(const void* p) {
+  WaveCtx& w = wv();
+  const int lane = blk->cur->lane, g = lane & 48, i = lane & 15;
+  w.ptr[lane] = p;
+  barrier_wait(w.bar);
+  uint16_t v[4];
+  for (int r = 0; r < 4; ++r) memcpy(&v[r], static_cast<const uint16_t*>(w.ptr[g + 4 * r + (i >> 2)]) + (i & 3), 2);
+  barrier_wait(w.bar);
+  uint2 o;
+  memcpy(&o, v, 8);
+  return o;
 }
 inline f16v mfma_32x32x2_f32(float a, float b, f16v c, int, int, int) {
   WaveCtx& w = wv();
@@ -585,6 +616,7 @@ inline void launch(dim3 grid, dim3 block, size_t lds_bytes, const std::function<
 #define __builtin_amdgcn_make_buffer_rsrc hipemu::make_rsrc
 #define __builtin_amdgcn_raw_buffer_load_b128 hipemu::raw_buffer_load_b128
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16 hipemu::mfma_32x32x16_f16
+#define __builtin_amdgcn_mfma_f32_32x32x16_bf16 hipemu::mfma_32x32x16_bf16
 #define __builtin_amdgcn_mfma_f32_32x32x2f32 hipemu::mfma_32x32x2_f32
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4 hipemu::mfma_scale_32x32x64_fp6
 #define __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32 hipemu::cvt_scalef32_2xpk16_fp6_f32

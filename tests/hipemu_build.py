@@ -54,3 +54,20 @@ def ensure():
         r = subprocess.run([CLANG, "-shared", "-fPIC", "-pthread", "-Wl,-Bsymbolic", "-Wl,--no-undefined", "-o", LIB] + objs, capture_output=True, text=True)
         assert r.returncode == 0, r.stderr[-3000:]
     return LIB
+
+
+def ensure_operators():
+    """libf5hip_operators_emu.so: the operators' entry points and kernels alone (operators_api.cpp, rotary.hip, window_attention.hip) for the host —
+    seconds to build where the whole engine takes minutes."""
+    csrc, emu = os.path.join(ROOT, "f5-tts_amd", "csrc"), os.path.join(ROOT, "tests", "hipemu")
+    lib = os.path.join(OUT, "libf5hip_operators_emu.so")
+    sources = [os.path.join(csrc, f) for f in ("rotary.hip", "window_attention.hip", "operators_api.cpp")] + [os.path.join(emu, "operators_error.cpp")]
+    deps = sources + [os.path.join(csrc, f) for f in ("common.h", "operators.h", "window_attention_kernel.h")] + \
+        [os.path.join(emu, "hipemu.h"), os.path.join(ROOT, "include", "f5hip.h")]
+    if not os.path.exists(lib) or any(os.path.getmtime(d) > os.path.getmtime(lib) for d in deps):
+        os.makedirs(OUT, exist_ok=True)
+        r = subprocess.run([CLANG, "-x", "c++", "-std=c++20", "-O1", "-pthread", "-fPIC", "-shared", "-DF5_HIPEMU", "-I", emu, "-I", csrc, "-Wno-unknown-pragmas",
+                            "-Wno-pass-failed", "-Wno-psabi", "-Wl,-Bsymbolic", "-Wl,--no-undefined", "-o", lib + ".part"] + sources, capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr[-3000:]
+        os.replace(lib + ".part", lib)
+    return lib

@@ -76,7 +76,11 @@ def attention(q, k, v, *, window=(-1, -1), sinks=0, kv_len=None, q_len=None, ali
             # each weight is off by e^ds - 1 and, in 16 bits, by its rounding; the sums over n keys by 2^-24 a step (two sums, and a merge
             # of parts); numerator and denominator each, hence mass + |o|; then the output's own rounding
             dw = torch.expm1(ds) + up + (n + 16) * 2.0 ** -24
-            tol[i, :m, head] = dw * (mass + o.abs()) * (1 + 2 * up) + ut * o.abs() + (2.0 ** -25 if q.dtype == torch.float16 else 0.0)
+            tol[i, :m, head] = dw * (mass + o.abs()) * (1 + 2 * up) + ut * o.abs()
+            if q.dtype == torch.float16:
+                # half a step among the subnormal numbers, 2^-25: of the output, and of each weight, which are held so that the row's
+                # largest is at least 2^7 (and their sum with it): 2^-32 of |v| for every key seen, in numerator and denominator
+                tol[i, :m, head] += 2.0 ** -25 + 2.0 ** -32 * (seen.double() @ z.abs() + seen.sum(-1, keepdim=True) * o.abs())
     return out, tol, rows
 
 

@@ -13,15 +13,26 @@ sys.path.insert(0, ROOT)
 sys.path.insert(0, os.path.join(ROOT, "tests"))
 import operators_oracle as O  # noqa: E402
 from f5_tts_amd import binding, ops  # noqa: E402
-from test_hipemu import CLANG, engine_emu_lib  # noqa: E402,F401
+import hipemu_build  # noqa: E402
 
+CLANG = hipemu_build.CLANG
 shim = pytest.mark.skipif(not os.path.exists(CLANG), reason="needs the ROCm host clang++")
 
 
+@pytest.fixture(scope="module")
+def operators_emu_lib():
+    lib = C.CDLL(hipemu_build.ensure_operators(), mode=C.RTLD_LOCAL)
+    for name, (res, args) in binding.SYMBOLS.items():
+        if hasattr(lib, name):
+            fn = getattr(lib, name)
+            fn.restype, fn.argtypes = res, args
+    return lib
+
+
 @pytest.fixture()
-def host(engine_emu_lib, monkeypatch):  # noqa: F811
+def host(operators_emu_lib, monkeypatch):
     """ops over the emulated library: CPU tensors are its device tensors."""
-    monkeypatch.setattr(ops, "load_library", lambda *a, **k: engine_emu_lib)
+    monkeypatch.setattr(ops, "load_library", lambda *a, **k: operators_emu_lib)
     monkeypatch.setattr(ops, "_device", lambda t: (0, 0))
     return ops
 
