@@ -19,32 +19,39 @@ from .binding import F5HipError, check, load_library
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # F5HIP_T_*
 _LAYOUTS = {"interleaved": 0, "half": 1}                          # F5HIP_ROTARY_*
+_ALIGN = {"start": 0, "end": 1}
 _SCALINGS = {None: 0, "none": 0, "linear": 1, "ntk": 2, "yarn": 3}  # F5HIP_ROPE_*
 _ROTARY = struct.Struct("@10if4P12qPP2q")   # f5hip_rotary_args
 _WINDOW = struct.Struct("@11if4P12q3Pq")    # f5hip_window_attention_args
 
 
+# The calls below take about as long on the host as the small launches do on the GPU: each check is one comparison where it passes.
 def _device(t: torch.Tensor) -> Tuple[int, int]:
     """(device ordinal, current stream) of a GPU tensor."""
     if not t.is_cuda:
         raise F5HipError("the operators need tensors on a HIP device (torch device type 'cuda'); there is no CPU path")
-    return t.device.index, torch.cuda.current_stream(t.device).cuda_stream
+    index = t.get_device()
+    return index, torch._C._cuda_getCurrentRawStream(index)  # torch.cuda.current_stream(device).cuda_stream without the Python objects (2 us)
 
 
-def _strides(t: torch.Tensor) -> Tuple[int, int, int]:
-    n, s = t.shape, t.stride()  # an axis of one element may carry any stride
-    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+def _strides(shape, stride) -> Tuple[int, int, int]:
+    return (stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0, stride[2] if shape[2] > 1 else 0)  # an axis of one element may carry any stride
 
 
-def _tensor(name: str, t: torch.Tensor, like: Optional[torch.Tensor] = None) -> None:
+def _tensor(name: str, t: torch.Tensor, dtype: Optional[torch.dtype] = None, device: Optional[torch.device] = None) -> None:
     if not isinstance(t, torch.Tensor) or t.dim() != 4:
         raise ValueError(f"{name}: a [batch, tokens, heads, head_dim] tensor is expected")
-    if t.dtype not in _TYPES:
-        raise ValueError(f"{name}: {t.dtype} is not one of float32, float16, bfloat16")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
-        raise ValueError(f"{name}: {t.dtype} on {t.device}, the first tensor is {like.dtype} on {like.device}")
+    if dtype is None:
+        if t.dtype not in _TYPES:
+            raise ValueError(f"{name}: {t.dtype} is not one of float32, float16, bfloat16")
+    elif t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, the first tensor is {dtype} on {device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the operators are for inference (use torch.no_grad())")
+
+
+def _empty(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _lengths(name: str, t: Optional[torch.Tensor], like: torch.Tensor) -> Optional[torch.Tensor]:
@@ -85,22 +92,28 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
     k rotate (the reference's ``pe_attn_head``).  ``inverse`` turns back (with amplitude 1 the inverse; in any case the operator's gradient).
     ``out``: ``(q', k')`` to write to — the inputs themselves, or tensors that share no memory with them."""
     _tensor("q", q)
+    dtype, where, shape = q.dtype, q.device, q.shape
     if layout not in _LAYOUTS:
         raise ValueError(f"layout {layout!r}: 'interleaved' or 'half' is expected")
-    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != q.device:
-        raise ValueError(f"inv_freq: a float64 vector on {q.device} is expected (rotary_frequencies)")
+    if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != where:
+        raise ValueError(f"inv_freq: a float64 vector on {where} is expected (rotary_frequencies)")
     inv_freq = inv_freq.contiguous()
-    b, n, h, d = q.shape
+    b, n, h, d = shape
+    hk = 0
     if k is not None:
-        _tensor("k", k, q)
-        if k.shape[:2] != q.shape[:2] or k.shape[3] != d:
-            raise ValueError(f"k is {tuple(k.shape)}, q {tuple(q.shape)}: batch, tokens and head_dim must agree")
-        if k.stride(3) != 1 and d > 1:
-            k = k.contiguous() if out is None else k
+        _tensor("k", k, dtype, where)
+        kshape = k.shape
+        hk = kshape[2]
+        if kshape[0] != b or kshape[1] != n or kshape[3] != d or hk == 0:
+            raise ValueError(f"k is {tuple(kshape)}, q {tuple(shape)}: batch, tokens and head_dim must agree")
     if out is None:
         q = q if q.stride(3) == 1 else q.contiguous()
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q_out = _empty(q)
+        if k is None:
+            k_out = None
+        else:
+            k = k if k.stride(3) == 1 else k.contiguous()
+            k_out = _empty(k)
     else:
         q_out, k_out = out
         for name, x, y in (("q", q, q_out), ("k", k, k_out)):
@@ -108,35 +121,40 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
                 raise ValueError(f"out: one tensor for q and one for k is expected, None for a {name} that is None")
             if x is None:
                 continue
-            _tensor(f"out for {name}", y, q)
+            _tensor(f"out for {name}", y, dtype, where)
             if y.shape != x.shape:
                 raise ValueError(f"out for {name} is {tuple(y.shape)}, {name} {tuple(x.shape)}")
             if x.stride(3) != 1 or y.stride(3) != 1:
                 raise ValueError(f"{name}: with out the last axis of input and output must be contiguous")
     step = 0
     if positions is not None:
-        if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int64 or positions.device != q.device or \
+        if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int64 or positions.device != where or \
                 tuple(positions.shape) not in ((n,), (1, n), (b, n)):
-            raise ValueError(f"positions: int64 of [tokens] or [batch, tokens] on {q.device} is expected")
+            raise ValueError(f"positions: int64 of [tokens] or [batch, tokens] on {where} is expected")
         positions = positions.contiguous()
         step = n if positions.dim() == 2 and positions.shape[0] > 1 else 0
     device, stream = _device(q)
-    args = _pack(_ROTARY, (_TYPES[q.dtype], _LAYOUTS[layout], int(bool(inverse)), 2 * inv_freq.shape[0], b, n, h, 0 if k is None else k.shape[2], d,
-                           -1 if rot_heads is None else rot_heads, amplitude, q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(),
-                           0 if k is None else k_out.data_ptr(), *_strides(q), *((0, 0, 0) if k is None else _strides(k)), *_strides(q_out),
-                           *((0, 0, 0) if k is None else _strides(k_out)), inv_freq.data_ptr(), 0 if positions is None else positions.data_ptr(),
-                           step, offset))
+    qs, qos = _strides(shape, q.stride()), _strides(shape, q_out.stride())
+    ks, kos, kp, kop = ((0, 0, 0), (0, 0, 0), 0, 0) if k is None else \
+        (_strides(kshape, k.stride()), _strides(kshape, k_out.stride()), k.data_ptr(), k_out.data_ptr())
+    args = _pack(_ROTARY, (_TYPES[dtype], _LAYOUTS[layout], 1 if inverse else 0, 2 * inv_freq.shape[0], b, n, h, hk, d,
+                           -1 if rot_heads is None else rot_heads, amplitude, q.data_ptr(), kp, q_out.data_ptr(), kop, *qs, *ks, *qos, *kos,
+                           inv_freq.data_ptr(), 0 if positions is None else positions.data_ptr(), step, offset))
     lib = load_library()
-    check(lib, None, lib.f5hip_rotary(args, device, stream))
+    status = lib.f5hip_rotary(args, device, stream)
+    if status:
+        check(lib, None, status)
     return q_out, k_out
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """The tensor, or a copy, with 16-byte aligned rows."""
-    e = t.element_size()
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any((s * e) % 16 for s in _strides(t)):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _rows(t: torch.Tensor, shape) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
+    """The tensor, or a copy, with 16-byte aligned rows, and its strides."""
+    stride = t.stride()
+    st = _strides(shape, stride)
+    if stride[3] == 1 and ((st[0] | st[1] | st[2]) * t.element_size() | t.data_ptr()) % 16 == 0:
+        return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, _strides(shape, t.stride())
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: Tuple[int, int] = (-1, -1), sinks: int = 0,
@@ -151,38 +169,44 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     ``out``.  ``scale``: 1 / sqrt(D) by default.  D: a multiple of 8 (fp32: 4) up to 128.  Keys and values that no query sees may hold
     anything; tensors whose rows are not aligned to 16 bytes are copied first."""
     _tensor("q", q)
-    _tensor("k", k, q)
-    _tensor("v", v, q)
-    b, n, h, d = q.shape
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: batch and head_dim must agree, k and v in all axes")
-    if d == 0 or h == 0 or k.shape[2] == 0:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}: heads and head_dim must be positive")
-    if align not in ("start", "end"):
+    dtype, where, shape = q.dtype, q.device, q.shape
+    _tensor("k", k, dtype, where)
+    _tensor("v", v, dtype, where)
+    b, n, h, d = shape
+    kshape = k.shape
+    if kshape != v.shape or kshape[0] != b or kshape[3] != d:
+        raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}, v {tuple(v.shape)}: batch and head_dim must agree, k and v in all axes")
+    if d == 0 or h == 0 or kshape[2] == 0:
+        raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}: heads and head_dim must be positive")
+    if align not in _ALIGN:
         raise ValueError(f"align {align!r}: 'start' or 'end' is expected")
     kv_len, q_len = _lengths("kv_len", kv_len, q), _lengths("q_len", q_len, q)
     left, right = window
     if out is None:
-        out = (torch.empty if q_len is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+        out = _empty(q) if q_len is None else torch.zeros(shape, dtype=dtype, device=where)
     else:
-        _tensor("out", out, q)
-        if out.shape != q.shape:
-            raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
+        _tensor("out", out, dtype, where)
+        if out.shape != shape:
+            raise ValueError(f"out is {tuple(out.shape)}, q {tuple(shape)}")
         if out.stride(3) != 1:
             raise ValueError("out: the last axis must be contiguous")
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    q, qs = _rows(q, shape)
+    k, ks = _rows(k, kshape)
+    v, vs = _rows(v, kshape)
     device, stream = _device(q)
     lib = load_library()
-    fields = [_TYPES[q.dtype], b, n, k.shape[1], h, k.shape[2], d, left, right, sinks, int(align == "end"), d ** -0.5 if scale is None else scale,
-              q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *_strides(q), *_strides(k), *_strides(v), *_strides(out),
+    fields = [_TYPES[dtype], b, n, kshape[1], h, kshape[2], d, left, right, sinks, _ALIGN[align], d ** -0.5 if scale is None else scale,
+              q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *qs, *ks, *vs, *_strides(shape, out.stride()),
               0 if kv_len is None else kv_len.data_ptr(), 0 if q_len is None else q_len.data_ptr(), 0, 0]
     args = _pack(_WINDOW, fields)
     need = lib.f5hip_window_attention_workspace(args)
     if need < 0:
         check(lib, None, 1)
     if need:
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        work = torch.empty(need, dtype=torch.uint8, device=where)
         fields[-2:] = [work.data_ptr(), need]
         args = _pack(_WINDOW, fields)
-    check(lib, None, lib.f5hip_window_attention(args, device, stream))
+    status = lib.f5hip_window_attention(args, device, stream)
+    if status:
+        check(lib, None, status)
     return out
