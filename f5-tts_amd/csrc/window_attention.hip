@@ -30,7 +30,7 @@ template <typename T>
 hipError_t launch(const WindowArgs& w, const Plan& p, hipStream_t s) {
   const auto go = [&](auto DP) {
     constexpr int dp = decltype(DP)::value;
-    if (p.few) hipLaunchKernelGGL((window_few_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(64 * FEW_WAVES), 0, s, w);
+    if (p.few) hipLaunchKernelGGL((window_few_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(64 * FEW_WAVES<T>), 0, s, w);
     else hipLaunchKernelGGL((window_rows_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
   };
   if (w.dim <= 64) go(std::integral_constant<int, 64>{});

@@ -63,7 +63,12 @@ struct Win<bf16> {
     return __builtin_bit_cast(uint32_t, v);
   }
   static __device__ __forceinline__ float add2(uint32_t p, float acc) {
+#ifdef F5_HIPEMU
     return acc + (__builtin_bit_cast(float, p << 16) + __builtin_bit_cast(float, p & 0xffff0000u));
+#else
+    const bf16x2 ones = {(bf16)1.0f, (bf16)1.0f};
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), ones, acc, false);
+#endif
   }
 };
 template <>
@@ -229,7 +234,7 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
   constexpr int KT = Win<T>::KT, NB = KT / 32, EB = R::EB, CPR = DP * EB / 16, NL = KT * CPR / 256;
   constexpr int VOFF = KT * R::K_ROWB, STAGE = VOFF + KT * R::V_ROWB;
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, ql = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, ql = lane & 31;
   int L = xcd_order((int)blockIdx.x, a.nwg);
   const int ks = L % a.nsplit;
   L /= a.nsplit;
@@ -269,6 +274,13 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
   const int64_t ksb = a.k_stride[1] * EB, vsb = a.v_stride[1] * EB;
   const int dimb = a.dim * EB;
   uint4 rk[NL], rv[NL];
+  uint32_t ok[NL], ov[NL];  // the thread's pieces of a tile (rows past its last key are past the descriptor's end, columns past the head's are put there)
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
+    ok[i] = col * 16 < dimb ? (uint32_t)(r * (int)ksb + col * 16) : OOB_ROW;
+    ov[i] = col * 16 < dimb ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW;
+  }
   const auto tile = [&](int t, int& key0, int& kend) {
     key0 = t < na ? t * KT : bb + (t - na) * KT;
     kend = t < na ? ea : khigh;
@@ -279,12 +291,9 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
     const int rows = min(KT, kend - key0);
     const BufRsrc Kr = tile_rsrc(kb, ksb, key0, rows, dimb), Vr = tile_rsrc(vb, vsb, key0, rows, dimb);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
-      const bool in = col * 16 < dimb && r < rows;
-      rk[i] = buffer_load_b128(Kr, in ? (uint32_t)(r * (int)ksb + col * 16) : OOB_ROW);
-      rv[i] = buffer_load_b128(Vr, in ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW);
-    }
+    for (int i = 0; i < NL; ++i) rk[i] = buffer_load_b128(Kr, ok[i]);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) rv[i] = buffer_load_b128(Vr, ov[i]);
   };
   const auto store = [&](int stage) {
     char* base = smem + stage * STAGE;
@@ -356,16 +365,18 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
 
 // ---- few rows: one 32-row group, the waves along the keys ----------------------------------------------------------------------------------------
 // Every wave walks 32-key tiles of its own (tile t belongs to wave t % NW): K straight into operand registers, V through the wave's own LDS rows, no
-// barrier on the way, the next tile's loads in flight meanwhile; the waves' results meet in LDS at the end, in a fixed order.
-constexpr int FEW_WAVES = 8;
+// barrier on the way, the next tile's loads issued as soon as the registers are free; the waves' results meet in LDS at the end, in a fixed order.
+// 8 waves; 4 in fp32, whose operands of one tile fill a 512-register wave.
+template <typename T>
+constexpr int FEW_WAVES = sizeof(T) == 4 ? 4 : 8;
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * FEW_WAVES, 1) void window_few_kernel(WindowArgs a) {
+__global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(WindowArgs a) {
   using R = Rows<T, DP>;
-  constexpr int NW = FEW_WAVES, KT = 32, EB = R::EB, CPR = DP * EB / 16, NL = KT * CPR / 64;
+  constexpr int NW = FEW_WAVES<T>, KT = 32, EB = R::EB, CPR = DP * EB / 16, NL = KT * CPR / 64;
   constexpr int VB = KT * R::V_ROWB, MERGE = NW * 32 * 33 * 4;
   __shared__ __attribute__((aligned(16))) char smem[NW * VB > MERGE ? NW * VB : MERGE];
   __shared__ float sml[NW][32][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, ql = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, ql = lane & 31;
   int L = xcd_order((int)blockIdx.x, a.nwg);
   const int ks = L % a.nsplit;
   L /= a.nsplit;
@@ -405,23 +416,34 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 1) void window_few_kernel(WindowArg
     key0 = t < na ? t * KT : bb + (t - na) * KT;
     kend = t < na ? ea : khigh;
   };
-  const auto load = [&](int t, uint4 (&fk)[R::NKS], uint4 (&rv)[NL]) {
+  uint4 fk[R::NKS], rv[NL];
+  uint32_t ok[R::NKS], ov[NL];
+#pragma unroll
+  for (int k = 0; k < R::NKS; ++k) ok[k] = k * 32 + half * 16 < dimb ? (uint32_t)(ql * (int)ksb + k * 32 + half * 16) : OOB_ROW;
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int c = lane + i * 64, r = c / CPR, col = c - r * CPR;
+    ov[i] = col * 16 < dimb ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW;
+  }
+  const auto load_k = [&](int t) {
     int key0, kend;
     tile(t, key0, kend);
-    const int rows = min(KT, kend - key0);
-    const BufRsrc Kr = tile_rsrc(kb, ksb, key0, rows, dimb), Vr = tile_rsrc(vb, vsb, key0, rows, dimb);
+    const BufRsrc Kr = tile_rsrc(kb, ksb, key0, min(KT, kend - key0), dimb);
 #pragma unroll
-    for (int k = 0; k < R::NKS; ++k) {
-      const int col = k * 32 + half * 16;
-      fk[k] = buffer_load_b128(Kr, col < dimb && ql < rows ? (uint32_t)(ql * (int)ksb + col) : OOB_ROW);
-    }
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int c = lane + i * 64, r = c / CPR, col = c - r * CPR;
-      rv[i] = buffer_load_b128(Vr, col * 16 < dimb && r < rows ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW);
-    }
+    for (int k = 0; k < R::NKS; ++k) fk[k] = buffer_load_b128(Kr, ok[k]);
   };
-  const auto process = [&](int t, const uint4 (&fk)[R::NKS], const uint4 (&rv)[NL]) {
+  const auto load_v = [&](int t) {
+    int key0, kend;
+    tile(t, key0, kend);
+    const BufRsrc Vr = tile_rsrc(vb, vsb, key0, min(KT, kend - key0), dimb);
+#pragma unroll
+    for (int i = 0; i < NL; ++i) rv[i] = buffer_load_b128(Vr, ov[i]);
+  };
+  if (t0 + wave < t1) {
+    load_k(t0 + wave);
+    load_v(t0 + wave);
+  }
+  for (int t = t0 + wave; t < t1; t += NW) {
     int key0, kend;
     tile(t, key0, kend);
     f32x16 s[1];
@@ -429,28 +451,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES, 1) void window_few_kernel(WindowArg
     for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
 #pragma unroll
     for (int k = 0; k < R::NKS; ++k) Win<T>::mma(s[0], fk[k], st.fq[k]);
-    wave_lds_sync();  // the last tile's reads of these rows come before
+    if (t + NW < t1) load_k(t + NW);  // as soon as its registers are free
+    wave_lds_sync();                  // the last tile's reads of these rows come before
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int c = lane + i * 64, r = c / CPR, col = c - r * CPR;
       *reinterpret_cast<uint4*>(sv + r * R::V_ROWB + col * 16) = rv[i];
     }
+    if (t + NW < t1) load_v(t + NW);
     const bool border = !(key0 + KT <= min(high0, kend) && (key0 >= low1 || key0 + KT <= a.sinks));
     st.softmax(s, key0, kend, half, border, a);
     wave_lds_sync();
     st.product(s, sv, lane);
-  };
-  uint4 k0[R::NKS], v0[NL], k1[R::NKS], v1[NL];
-  int t = t0 + wave;
-  if (t < t1) load(t, k0, v0);
-  while (t < t1) {
-    if (t + NW < t1) load(t + NW, k1, v1);
-    process(t, k0, v0);
-    t += NW;
-    if (t >= t1) break;
-    if (t + NW < t1) load(t + NW, k0, v0);
-    process(t, k1, v1);
-    t += NW;
   }
 
   // the waves' parts: common reference, then 32 columns at a time through LDS, summed in the waves' order
