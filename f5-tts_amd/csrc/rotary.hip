@@ -2,10 +2,11 @@
 //
 // (x, y) -> a (x cos - y sin, x sin + y cos) with the angle p f_i: three flops a value against 4 (16-bit types) to 8 (fp32) bytes moved, so
 // the operator is a copy that computes on the way.  A thread owns one piece of a head's columns (16 bytes where sizes and alignment allow:
-// VEC elements of both members of its pairs) at one token, and walks over the heads of q and then of k in steps of `hg`: its sines and cosines are
-// computed once for all of them.  Consecutive threads take consecutive pieces, then consecutive heads, so a wave's access is one contiguous
+// VEC elements of both members of its pairs) at one token, in up to four of the heads of q and k, `hg` apart.  Consecutive threads take consecutive pieces, then consecutive heads, so a wave's access is one contiguous
 // run wherever the heads are.  Heads per thread grow with the size of the call (launch_rotary): one at a time for single tokens, where only
-// the number of threads hides latency, up to eight where the chip is full and the angle work is worth sharing.
+// the number of threads hides latency, up to four where the chip is full and the loads of several heads in flight are worth their registers.
+// A workgroup's threads cover a few tokens; it works out each of their angles once, while its loads are under way, and hands the cosines and sines
+// round through LDS (eight angles a thread by itself cost 2000 cycles and 100 registers: 4 x 8192 tokens of 40 heads of 128 took 176 us).
 //
 // The angle: turns t = p f / 2 pi in 64 bits, reduced to t - rint(t) in [-1/2, 1/2] in 64 bits (at p = 2^31 the product is 2^-22 turns exact),
 // then sin / cos of pi times twice that in fp32.  In fp32 from the start the product alone would be off by 2^-24 p f radians: 0.008 at
@@ -36,75 +37,85 @@ struct alignas(sizeof(T) * N) Piece {
 };
 
 // TWO = false: an item is VEC / 2 interleaved pairs in one piece.  TWO = true: an item is VEC first members and, off_b columns on, their
-// partners (the half layout; also, with VEC = 1, interleaved pairs that are not aligned to be read together).  U heads are loaded before
-// the first of them is stored: an output may be its input, so the compiler does not move a load over a store by itself.
+// partners (the half layout; also, with VEC = 1, interleaved pairs that are not aligned to be read together).  The thread's U heads, hg apart, are
+// loaded before its angles are worked out and before the first is stored (an output may be its input, so the compiler moves no load over a store).
 template <typename T, int VEC, bool TWO, int U>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   using P = Piece<T, VEC>;
   constexpr int NP = TWO ? VEC : VEC / 2;  // pairs of an item
+  F5_DYN_LDS(float2, turns_lds);  // [tokens of the workgroup][rot / 2] (cos, sin)
   const uint32_t slots = (uint32_t)a.nitem * (uint32_t)a.hg;
   const uint32_t id = blockIdx.x * 256u + threadIdx.x, token = id / slots;
-  if (token >= (uint32_t)a.tokens) return;
+  const uint32_t token0 = blockIdx.x * 256u / slots, token1 = min((blockIdx.x * 256u + 255u) / slots, (uint32_t)a.tokens - 1u);
+  const bool exists = token < (uint32_t)a.tokens;
+  const int half_rot = a.rot / 2, nangle = (int)(token1 - token0 + 1u) * half_rot;
   const uint32_t slot = id - token * slots;
   const int h0 = (int)(slot / (uint32_t)a.nitem), item = (int)(slot - (uint32_t)h0 * (uint32_t)a.nitem);
   const bool pair = item < a.npair;
   const int col = pair ? item * a.step : a.rot + (item - a.npair) * VEC;
   for (int b = blockIdx.y; b < a.batch; b += gridDim.y) {
+    P x[U], y[U];
+    bool turn[U], live[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + u * a.hg;
+      const bool isq = h < a.heads_q;
+      const int hh = isq ? h : h - a.heads_q;
+      turn[u] = pair && hh < (isq ? a.turned_q : a.turned_k);
+      live[u] = exists && h < a.heads && (turn[u] || !(isq ? a.keep_q : a.keep_k));
+      if (!live[u]) continue;
+      const int64_t* st = isq ? a.q_stride : a.k_stride;
+      const T* in = static_cast<const T*>(isq ? a.q : a.k) + b * st[0] + (int64_t)token * st[1] + hh * st[2] + col;
+      x[u] = *reinterpret_cast<const P*>(in);
+      if (TWO && pair) y[u] = *reinterpret_cast<const P*>(in + a.off_b);
+    }
+    for (int i = threadIdx.x; i < nangle; i += 256) {
+      const int t = i / half_rot, f = i - t * half_rot;
+      const int64_t tok = (int64_t)token0 + t, p = a.positions ? a.positions[(int64_t)b * a.position_stride + tok] : a.first + tok;
+      const double turns = (double)p * (a.inv_freq[f] * 0.15915494309189533577);  // 1 / 2 pi
+      const double r = turns - rint(turns);
+      float2 cs;
+#ifdef F5_HIPEMU
+      cs.x = (float)cos(6.283185307179586477 * r);
+      cs.y = (float)sin(6.283185307179586477 * r);
+#else
+      sincospif(2.0f * (float)r, &cs.y, &cs.x);
+#endif
+      cs.x *= a.amplitude;
+      cs.y *= a.amplitude * a.sign;
+      turns_lds[i] = cs;
+    }
+    __syncthreads();
     float c[NP], s[NP];
-    if (pair) {
-      const int64_t p = a.positions ? a.positions[(int64_t)b * a.position_stride + token] : a.first + (int64_t)token;
+    if (pair && exists) {
+      const float2* at = turns_lds + (token - token0) * (uint32_t)half_rot + item * NP;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const double turns = (double)p * (a.inv_freq[item * NP + i] * 0.15915494309189533577);  // 1 / 2 pi
-        const double r = turns - rint(turns);
-#ifdef F5_HIPEMU
-        c[i] = (float)cos(6.283185307179586477 * r);
-        s[i] = (float)sin(6.283185307179586477 * r);
-#else
-        sincospif(2.0f * (float)r, &s[i], &c[i]);
-#endif
-        c[i] *= a.amplitude;
-        s[i] *= a.amplitude * a.sign;
+        c[i] = at[i].x;
+        s[i] = at[i].y;
       }
     }
-    for (int h = h0; h < a.heads; h += U * a.hg) {
-      P x[U], y[U];
-      T* out[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int hu = h + u * a.hg;
-        out[u] = nullptr;
-        if (hu >= a.heads) continue;
-        const bool isq = hu < a.heads_q;
-        const int hh = isq ? hu : hu - a.heads_q;
-        const bool turn = pair && hh < (isq ? a.turned_q : a.turned_k);
-        if (!turn && (isq ? a.keep_q : a.keep_k)) continue;
-        const int64_t* si = isq ? a.q_stride : a.k_stride;
-        const int64_t* so = isq ? a.q_out_stride : a.k_out_stride;
-        const T* in = static_cast<const T*>(isq ? a.q : a.k) + b * si[0] + (int64_t)token * si[1] + hh * si[2] + col;
-        out[u] = static_cast<T*>(isq ? a.q_out : a.k_out) + b * so[0] + (int64_t)token * so[1] + hh * so[2] + col;
-        x[u] = *reinterpret_cast<const P*>(in);
-        if (TWO && pair) y[u] = *reinterpret_cast<const P*>(in + a.off_b);
-      }
+    for (int u = 0; u < U; ++u) {
+      if (!live[u]) continue;
+      const int h = h0 + u * a.hg;
+      const bool isq = h < a.heads_q;
+      if (turn[u]) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!out[u]) continue;
-        const int hu = h + u * a.hg;
-        const bool turn = pair && (hu < a.heads_q ? hu < a.turned_q : hu - a.heads_q < a.turned_k);
-        if (turn) {
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            T& tx = x[u].v[TWO ? i : 2 * i];
-            T& ty = TWO ? y[u].v[i] : x[u].v[TWO ? i : 2 * i + 1];
-            const float fx = (float)tx, fy = (float)ty;
-            tx = (T)(fx * c[i] - fy * s[i]);  // rounded once, to the nearest
-            ty = (T)(fx * s[i] + fy * c[i]);
-          }
+        for (int i = 0; i < NP; ++i) {
+          T& tx = x[u].v[TWO ? i : 2 * i];
+          T& ty = TWO ? y[u].v[i] : x[u].v[TWO ? i : 2 * i + 1];
+          const float fx = (float)tx, fy = (float)ty;
+          tx = (T)(fx * c[i] - fy * s[i]);  // rounded once, to the nearest
+          ty = (T)(fx * s[i] + fy * c[i]);
         }
-        *reinterpret_cast<P*>(out[u]) = x[u];
-        if (TWO && pair) *reinterpret_cast<P*>(out[u] + a.off_b) = y[u];
       }
+      const int64_t* st = isq ? a.q_out_stride : a.k_out_stride;
+      T* out = static_cast<T*>(isq ? a.q_out : a.k_out) + b * st[0] + (int64_t)token * st[1] + (isq ? h : h - a.heads_q) * st[2] + col;
+      *reinterpret_cast<P*>(out) = x[u];
+      if (TWO && pair) *reinterpret_cast<P*>(out + a.off_b) = y[u];
     }
+    __syncthreads();  // the next sequence's angles take the place of these
   }
 }
 
@@ -112,15 +123,19 @@ template <typename T, int VEC, bool TWO>
 hipError_t launch(RotaryArgs& r, int head_dim, hipStream_t s) {
   r.npair = TWO ? r.rot / 2 / VEC : r.rot / VEC;
   r.nitem = r.npair + (head_dim - r.rot) / VEC;
-  // Heads per thread: one until the call has more items than the chip keeps in flight (256 CUs x 2048 threads / 4), then up to eight.
+  // Heads per thread: one until the call has more items than a quarter of the chip's threads (256 CUs x 2048), then two, then four.
   const int64_t items = (int64_t)r.batch * r.tokens * r.heads * r.nitem;
-  const int per = (int)std::max<int64_t>(1, std::min<int64_t>(8, items / (256 * 512)));
+  const int per = items < 256 * 1024 ? 1 : items < 256 * 2048 ? 2 : 4;
   r.hg = (r.heads + per - 1) / per;
   const int64_t threads = (int64_t)r.tokens * r.nitem * r.hg;
   if (threads > 0x7fffff00) return hipErrorInvalidValue;
   const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)std::min(r.batch, 65535));
-  if (per == 1) hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 1>), grid, dim3(256), 0, s, r);
-  else hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 4>), grid, dim3(256), 0, s, r);
+  // 256 threads touch at most 256 / slots + 2 tokens: 48 KiB for the largest head, under 17 KiB for the smallest
+  const int64_t slots = (int64_t)r.nitem * r.hg;
+  const size_t lds = (size_t)(256 / slots + 2) * (r.rot / 2) * sizeof(float2);
+  if (per == 1) hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 1>), grid, dim3(256), lds, s, r);
+  else if (per == 2) hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 2>), grid, dim3(256), lds, s, r);
+  else hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 4>), grid, dim3(256), lds, s, r);
   return hipGetLastError();
 }
 
