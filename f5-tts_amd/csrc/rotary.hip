@@ -2,11 +2,12 @@
 //
 // (x, y) -> a (x cos - y sin, x sin + y cos) with the angle p f_i: three flops a value against 4 (16-bit types) to 8 (fp32) bytes moved, so
 // the operator is a copy that computes on the way.  A thread owns one piece of a head's columns (16 bytes where sizes and alignment allow:
-// VEC elements of both members of its pairs) at one token, in up to four of the heads of q and k, `hg` apart.  Consecutive threads take consecutive pieces, then consecutive heads, so a wave's access is one contiguous
-// run wherever the heads are.  Heads per thread grow with the size of the call (launch_rotary): one at a time for single tokens, where only
-// the number of threads hides latency, up to four where the chip is full and the loads of several heads in flight are worth their registers.
+// VEC elements of both members of its pairs) at one token, in one or two of the heads of q and k, `hg` apart.  Consecutive threads take
+// consecutive pieces, then consecutive heads, so a wave's access is one contiguous run wherever the heads are.  Heads per thread grow with the size of the call (launch_rotary): one at a time for single tokens, where only
+// the number of threads hides latency, two where the chip is full.
 // A workgroup's threads cover a few tokens; it works out each of their angles once, while its loads are under way, and hands the cosines and sines
-// round through LDS (eight angles a thread by itself cost 2000 cycles and 100 registers: 4 x 8192 tokens of 40 heads of 128 took 176 us).
+// round through LDS (eight angles a thread by itself cost 2000 cycles and 100 registers: 4 x 8192 tokens of 40 heads of 128 took 176 us; now 134 us,
+// 5.0 TB/s, which is what a large copy reaches on this card).
 //
 // The angle: turns t = p f / 2 pi in 64 bits, reduced to t - rint(t) in [-1/2, 1/2] in 64 bits (at p = 2^31 the product is 2^-22 turns exact),
 // then sin / cos of pi times twice that in fp32.  In fp32 from the start the product alone would be off by 2^-24 p f radians: 0.008 at
@@ -35,6 +36,21 @@ template <typename T, int N>
 struct alignas(sizeof(T) * N) Piece {
   T v[N];
 };
+
+// Stores past the cache: each XCD's L2 is written back at the kernel's end and whoever reads the output next sits on any XCD, so keeping it there buys
+// nothing (4 x 8192 tokens of 40 heads of 128: 144 us with ordinary stores, 134 us with these).
+template <typename P>
+__device__ __forceinline__ void store_past_cache(P* p, const P& v) {
+#ifdef F5_HIPEMU
+  *p = v;
+#else
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  using W = std::conditional_t<sizeof(P) == 16, u32x4, std::conditional_t<sizeof(P) == 8, u32x2, std::conditional_t<sizeof(P) == 4, unsigned, unsigned short>>>;
+  static_assert(sizeof(W) == sizeof(P), "pieces of 2 to 16 bytes");
+  __builtin_nontemporal_store(__builtin_bit_cast(W, v), reinterpret_cast<W*>(p));
+#endif
+}
 
 // TWO = false: an item is VEC / 2 interleaved pairs in one piece.  TWO = true: an item is VEC first members and, off_b columns on, their
 // partners (the half layout; also, with VEC = 1, interleaved pairs that are not aligned to be read together).  The thread's U heads, hg apart, are
@@ -112,8 +128,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
       }
       const int64_t* st = isq ? a.q_out_stride : a.k_out_stride;
       T* out = static_cast<T*>(isq ? a.q_out : a.k_out) + b * st[0] + (int64_t)token * st[1] + (isq ? h : h - a.heads_q) * st[2] + col;
-      *reinterpret_cast<P*>(out) = x[u];
-      if (TWO && pair) *reinterpret_cast<P*>(out + a.off_b) = y[u];
+      store_past_cache(reinterpret_cast<P*>(out), x[u]);
+      if (TWO && pair) store_past_cache(reinterpret_cast<P*>(out + a.off_b), y[u]);
     }
     __syncthreads();  // the next sequence's angles take the place of these
   }
@@ -123,9 +139,10 @@ template <typename T, int VEC, bool TWO>
 hipError_t launch(RotaryArgs& r, int head_dim, hipStream_t s) {
   r.npair = TWO ? r.rot / 2 / VEC : r.rot / VEC;
   r.nitem = r.npair + (head_dim - r.rot) / VEC;
-  // Heads per thread: one until the call has more items than a quarter of the chip's threads (256 CUs x 2048), then two, then four.
+  // Heads per thread: one until the call has half as many items as the chip holds threads (256 CUs x 2048), two above (4 x 8192 tokens of 40 heads of
+  // 128: 134 us, with four heads and their registers 139 us, with one 135 us; 2 x 1406 tokens of 32 heads of 64: 6.6, 7.8, 7.6 us).
   const int64_t items = (int64_t)r.batch * r.tokens * r.heads * r.nitem;
-  const int per = items < 256 * 1024 ? 1 : items < 256 * 2048 ? 2 : 4;
+  const int per = items < 256 * 1024 ? 1 : 2;
   r.hg = (r.heads + per - 1) / per;
   const int64_t threads = (int64_t)r.tokens * r.nitem * r.hg;
   if (threads > 0x7fffff00) return hipErrorInvalidValue;
@@ -134,8 +151,7 @@ hipError_t launch(RotaryArgs& r, int head_dim, hipStream_t s) {
   const int64_t slots = (int64_t)r.nitem * r.hg;
   const size_t lds = (size_t)(256 / slots + 2) * (r.rot / 2) * sizeof(float2);
   if (per == 1) hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 1>), grid, dim3(256), lds, s, r);
-  else if (per == 2) hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 2>), grid, dim3(256), lds, s, r);
-  else hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 4>), grid, dim3(256), lds, s, r);
+  else hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 2>), grid, dim3(256), lds, s, r);
   return hipGetLastError();
 }
 
