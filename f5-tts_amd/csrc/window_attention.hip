@@ -8,13 +8,15 @@ namespace {
 // into ranges where the row blocks alone leave CUs idle; both kernels then leave partial results that window_join_kernel merges.
 struct Plan {
   bool few;
+  int groups;  // many rows: 32-row groups of a wave
   int nblk, nsplit;
 };
 Plan plan_of(const f5hip_window_attention_args& a) {
   const int64_t rows = (int64_t)a.q_tokens * (a.heads / a.kv_heads), heads = (int64_t)a.batch * a.kv_heads;
   Plan p;
   p.few = rows <= 32;
-  const int per = p.few ? 32 : 128;
+  p.groups = !p.few && a.dtype != F5HIP_T_FP32 && a.head_dim <= 64 && heads * ((rows + 255) / 256) >= 512 ? 2 : 1;
+  const int per = p.few ? 32 : 128 * p.groups;
   p.nblk = (int)((rows + per - 1) / per);
   // the most keys a row block can see
   const int64_t tokens = std::min<int64_t>(a.q_tokens, per / (a.heads / a.kv_heads) + 2);
@@ -31,7 +33,8 @@ hipError_t launch(const WindowArgs& w, const Plan& p, hipStream_t s) {
   const auto go = [&](auto DP) {
     constexpr int dp = decltype(DP)::value;
     if (p.few) hipLaunchKernelGGL((window_few_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(64 * FEW_WAVES<T>), 0, s, w);
-    else hipLaunchKernelGGL((window_rows_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
+    else if (p.groups == 1) hipLaunchKernelGGL((window_rows_kernel<T, dp, 1>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
+    else if constexpr (sizeof(T) == 2 && dp == 64) hipLaunchKernelGGL((window_rows_kernel<T, dp, 2>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
   };
   if (w.dim <= 64) go(std::integral_constant<int, 64>{});
   else if (w.dim <= 96) go(std::integral_constant<int, 96>{});

@@ -40,7 +40,6 @@ template <typename T>
 struct Win;  // what differs between the element types
 template <>
 struct Win<f16> {
-  static constexpr int KT = 64;
   static constexpr float BIAS = 7.0f;
   static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -53,7 +52,6 @@ struct Win<f16> {
 };
 template <>
 struct Win<bf16> {
-  static constexpr int KT = 64;
   static constexpr float BIAS = 0.0f;
   static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -73,7 +71,6 @@ struct Win<bf16> {
 };
 template <>
 struct Win<float> {
-  static constexpr int KT = 32;
   static constexpr float BIAS = 0.0f;
   static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
     Frag x, y;
@@ -140,20 +137,31 @@ struct Rows {
     l = 0.f;
   }
 
-  // scores of NB blocks of 32 keys -> weights: mask (where `border`), reference maximum, exponentials, row sum
+  // the keys of NB blocks of 32 that the lane's row does not see -> -inf.  `high`, `low`, `sink` (wave-uniform): which borders the tile can
+  // touch — one compare and one select a score for each.
   template <int NB>
-  __device__ __forceinline__ void softmax(f32x16 (&s)[NB], int key0, int kend, int half, bool border, const WindowArgs& a) {
-    const float c = a.scale_log2;
-    if (border) {
-      const int base = key0 + 4 * half, e = min(hi, kend) - base, b = lo - base, k = a.sinks - base;
+  __device__ __forceinline__ void mask(f32x16 (&s)[NB], int key0, int kend, int half, bool high, bool low, int sinks) {
+    const int base = key0 + 4 * half, e = min(hi, kend) - base, b = lo - base, k = sinks - base;
+    if (high) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[n][r] = n * 32 + (r & 3) + 8 * (r >> 2) < e ? s[n][r] : -INFINITY;
+    }
+    if (low) {
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int off = n * 32 + (r & 3) + 8 * (r >> 2);
-          s[n][r] = (off < e) & ((off >= b) | (off < k)) ? s[n][r] : -INFINITY;
+          s[n][r] = ((off >= b) | (off < k)) ? s[n][r] : -INFINITY;
         }
     }
+  }
+
+  // the reference maximum, raised (and O, l rescaled) where the tile goes far above it
+  template <int NB>
+  __device__ __forceinline__ void raise(const f32x16 (&s)[NB], float c) {
     float mx = s[0][0];
 #pragma unroll
     for (int n = 0; n < NB; ++n)
@@ -171,44 +179,59 @@ struct Rows {
       m = mn;
       mc = mnc;
     }
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[n][r] = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -mc));
   }
 
-  // O^T += V^T P^T over NB blocks of 32 keys whose V rows lie at sv
-  template <int NB>
-  __device__ __forceinline__ void product(const f32x16 (&s)[NB], const char* sv, int lane) {
+  // A tile is worked through in phases, PHASES_PER_BLOCK for each 32 keys: 16 keys a phase in 16-bit types (the lane's are 16 g + 4 half + 0..3
+  // and 8 on), 8 in fp32 (four registers).  V^T operands of a phase, from V rows at sv:
+  static constexpr int PHASES_PER_BLOCK = EB == 2 ? 2 : 4;
+  struct VFrag {
+    uint4 v[ND];  // 16-bit types: 8 keys of a column; fp32: one key of a column for each of the phase's four registers
+  };
+  __device__ __forceinline__ void read_v(VFrag& f, int g, const char* sv, int lane) const {
     const int half = lane >> 5;
     if constexpr (EB == 2) {
-      const char* at = sv + (4 * half + ((lane & 15) >> 2)) * V_ROWB + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+      const char* at = sv + (4 * half + ((lane & 15) >> 2)) * V_ROWB + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2 + g * 16 * V_ROWB;
 #pragma unroll
-      for (int g = 0; g < 2 * NB; ++g) {  // 16 keys: the lane's are 16 g + 4 half + 0..3 and 8 on
-        uint32_t p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = Win<T>::pack(s[g >> 1][8 * (g & 1) + 2 * e], s[g >> 1][8 * (g & 1) + 2 * e + 1]);
-          l = Win<T>::add2(p[e], l);  // the sum is that of the rounded weights: numerator and denominator see the same ones
-        }
-        const uint4 fp = make_uint4(p[0], p[1], p[2], p[3]);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const uint2 v0 = lds_read_transposed(at + g * 16 * V_ROWB + d * 64), v1 = lds_read_transposed(at + (g * 16 + 8) * V_ROWB + d * 64);
-          Win<T>::mma(o[d], make_uint4(v0.x, v0.y, v1.x, v1.y), fp);
-        }
+      for (int d = 0; d < ND; ++d) {
+        const uint2 v0 = lds_read_transposed(at + d * 64), v1 = lds_read_transposed(at + 8 * V_ROWB + d * 64);
+        f.v[d] = make_uint4(v0.x, v0.y, v1.x, v1.y);
       }
     } else {
-      const char* at = sv + 4 * half * V_ROWB + (lane & 31) * 4;
+      const char* at = sv + (4 * half + 8 * g) * V_ROWB + (lane & 31) * 4;
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int d = 0; d < ND; ++d) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(at + d * 128);
+        f.v[d] = make_uint4(w[0], w[V_ROWB / 4], w[2 * V_ROWB / 4], w[3 * V_ROWB / 4]);
+      }
+    }
+  }
+  // the weights of phase g's keys, and O^T += V^T P^T over them
+  template <int NB>
+  __device__ __forceinline__ void weigh(const f32x16 (&s)[NB], int g, float c, const VFrag& f) {
+    if constexpr (EB == 2) {
+      uint32_t p[4];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          l += s[n][r];
+      for (int e = 0; e < 4; ++e) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * e], c, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * e + 1], c, -mc));
+        p[e] = Win<T>::pack(x, y);
+        l = Win<T>::add2(p[e], l);  // the sum is that of the rounded weights: numerator and denominator see the same ones
+      }
+      const uint4 fp = make_uint4(p[0], p[1], p[2], p[3]);
 #pragma unroll
-          for (int d = 0; d < ND; ++d)
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(at + (n * 32 + (r & 3) + 8 * (r >> 2)) * V_ROWB + d * 128), s[n][r], o[d], 0, 0, 0);
-        }
+      for (int d = 0; d < ND; ++d) Win<T>::mma(o[d], f.v[d], fp);
+    } else {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = __builtin_amdgcn_exp2f(fmaf(s[g >> 2][4 * (g & 3) + e], c, -mc));
+        l += w[e];
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const uint32_t v[4] = {f.v[d].x, f.v[d].y, f.v[d].z, f.v[d].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, v[e]), w[e], o[d], 0, 0, 0);
+      }
     }
   }
 };
@@ -227,50 +250,69 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (b >> 3);
 }
 
-// ---- many rows: 4 waves x 32 rows, K and V tiles shared through LDS, two stages --------------------------------------------------------------
-template <typename T, int DP>
+// ---- many rows: 4 waves x RT groups of 32 rows, K and V tiles shared through LDS, two stages ------------------------------------------------------
+// The tiles of a row block in order: keys [0, ea), then [bb, high).  One cursor walks them for the loads, one for the work; advancing costs a few scalar
+// instructions where indexing by a tile number took ninety.
+struct Tiles {
+  int key0, kend;  // the tile's first key, its range's end
+  int bb, high;
+  template <int KT>
+  __device__ __forceinline__ void next() {
+    key0 += KT;
+    if (key0 >= kend && kend != high) { key0 = bb; kend = high; }
+  }
+};
+
+template <typename T, int DP, int RT>
 __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
   using R = Rows<T, DP>;
-  constexpr int KT = Win<T>::KT, NB = KT / 32, EB = R::EB, CPR = DP * EB / 16, NL = KT * CPR / 256;
-  constexpr int VOFF = KT * R::K_ROWB, STAGE = VOFF + KT * R::V_ROWB;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+  constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32, EB = R::EB, CPR = DP * EB / 16, NP = KT * CPR, NL = (NP + 255) / 256, ROWS = 128 * RT;
+  constexpr int KB = KT * R::K_ROWB, VB = KT * R::V_ROWB;
+  __shared__ __attribute__((aligned(16))) char smem[2 * (KB + VB)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, ql = lane & 31;
   int L = xcd_order((int)blockIdx.x, a.nwg);
   const int ks = L % a.nsplit;
   L /= a.nsplit;
   const int blk = L % a.nblk, bh = L / a.nblk, b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
   const int n = a.kv_len ? max(0, min(a.kv_len[b], a.tk)) : a.tk, nq = a.q_len ? max(0, min(a.q_len[b], a.tq)) : a.tq;
-  const int first = blk * 128 / a.group;
+  const int first = blk * ROWS / a.group;
   if (first >= nq) return;  // (the whole workgroup: no barrier has been reached)
   const int p0 = a.align_end ? n - nq : 0;
   const Span sp{n, a.left, a.right};
-  const int last = min(nq - 1, (blk * 128 + 127) / a.group);
+  const int last = min(nq - 1, (blk * ROWS + ROWS - 1) / a.group);
   const int khigh = sp.high(p0 + last), klow = min(sp.low(p0 + first), khigh), ksink = min(a.sinks, khigh);
   const int ea = klow <= ksink ? 0 : ksink, bb = klow <= ksink ? 0 : klow;  // keys [0, ea) and [bb, khigh)
   const int na = (ea + KT - 1) / KT, nt = na + (khigh - bb + KT - 1) / KT;
   const int t0 = (int)((int64_t)ks * nt / a.nsplit), t1 = (int)((int64_t)(ks + 1) * nt / a.nsplit);
 
-  // the wave's rows, the lane's row
-  const int row = blk * 128 + wave * 32 + ql, tok = row / a.group, g = row - tok * a.group, head = kvh * a.group + g;
-  const bool live = tok < nq;
-  const int wfirst = min(nq - 1, (blk * 128 + wave * 32) / a.group), wlast = min(nq - 1, (blk * 128 + wave * 32 + 31) / a.group);
-  const bool idle = (blk * 128 + wave * 32) / a.group >= nq;
-  const int whi0 = sp.high(p0 + wfirst), whi1 = sp.high(p0 + wlast), wlo0 = sp.low(p0 + wfirst), wlo1 = sp.low(p0 + wlast);
-  R st;
-  st.reset();
-  st.lo = sp.low(p0 + tok);
-  st.hi = live ? sp.high(p0 + tok) : 0;
-  const T* qp = static_cast<const T*>(a.q) + b * a.q_stride[0] + tok * a.q_stride[1] + head * a.q_stride[2];
+  // the wave's rows: RT groups of 32, a lane's row in each
+  R st[RT];
+  const T* qp[RT];
+  int tok[RT], head[RT], whi0[RT], whi1[RT], wlo0[RT], wlo1[RT];
 #pragma unroll
-  for (int k = 0; k < R::NKS; ++k) {
-    const int col = (k * 32 + half * 16) / EB;
-    uint4 u = live && col < a.dim ? *reinterpret_cast<const uint4*>(qp + col) : make_uint4(0, 0, 0, 0);
-    u.x ^= a.negate; u.y ^= a.negate; u.z ^= a.negate; u.w ^= a.negate;
-    st.fq[k] = u;
+  for (int x = 0; x < RT; ++x) {
+    const int r0 = blk * ROWS + (wave * RT + x) * 32, row = r0 + ql;
+    tok[x] = row / a.group;
+    head[x] = kvh * a.group + (row - tok[x] * a.group);
+    const int wfirst = r0 / a.group, wlast = min(nq - 1, (r0 + 31) / a.group);
+    // the tightest and widest borders of the group's rows; no row at all: nothing is seen
+    whi0[x] = sp.high(p0 + wfirst);
+    whi1[x] = wfirst < nq ? sp.high(p0 + wlast) : 0;
+    wlo0[x] = sp.low(p0 + wfirst);
+    wlo1[x] = sp.low(p0 + wlast);
+    st[x].reset();
+    st[x].lo = sp.low(p0 + tok[x]);
+    st[x].hi = tok[x] < nq ? sp.high(p0 + tok[x]) : 0;
+    qp[x] = static_cast<const T*>(a.q) + b * a.q_stride[0] + tok[x] * a.q_stride[1] + head[x] * a.q_stride[2];
+#pragma unroll
+    for (int k = 0; k < R::NKS; ++k) {
+      const int col = (k * 32 + half * 16) / EB;
+      uint4 u = tok[x] < nq && col < a.dim ? *reinterpret_cast<const uint4*>(qp[x] + col) : make_uint4(0, 0, 0, 0);
+      u.x ^= a.negate; u.y ^= a.negate; u.z ^= a.negate; u.w ^= a.negate;
+      st[x].fq[k] = u;
+    }
   }
 
-  const char* kb = static_cast<const char*>(a.k) + (b * a.k_stride[0] + kvh * a.k_stride[2]) * EB;
-  const char* vb = static_cast<const char*>(a.v) + (b * a.v_stride[0] + kvh * a.v_stride[2]) * EB;
   const int64_t ksb = a.k_stride[1] * EB, vsb = a.v_stride[1] * EB;
   const int dimb = a.dim * EB;
   uint4 rk[NL], rv[NL];
@@ -278,89 +320,117 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
     const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
-    ok[i] = col * 16 < dimb ? (uint32_t)(r * (int)ksb + col * 16) : OOB_ROW;
-    ov[i] = col * 16 < dimb ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW;
+    const bool in = col * 16 < dimb && (NP % 256 == 0 || c < NP);
+    ok[i] = in ? (uint32_t)(r * (int)ksb + col * 16) : OOB_ROW;
+    ov[i] = in ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW;
   }
-  const auto tile = [&](int t, int& key0, int& kend) {
-    key0 = t < na ? t * KT : bb + (t - na) * KT;
-    kend = t < na ? ea : khigh;
-  };
-  const auto load = [&](int t) {
-    int key0, kend;
-    tile(t, key0, kend);
-    const int rows = min(KT, kend - key0);
-    const BufRsrc Kr = tile_rsrc(kb, ksb, key0, rows, dimb), Vr = tile_rsrc(vb, vsb, key0, rows, dimb);
+  const char* kb = static_cast<const char*>(a.k) + (b * a.k_stride[0] + kvh * a.k_stride[2]) * EB;
+  const char* vb = static_cast<const char*>(a.v) + (b * a.v_stride[0] + kvh * a.v_stride[2]) * EB;
+  const auto load = [&](const Tiles& t) {
+    const int rows = min(KT, t.kend - t.key0);
+    const BufRsrc Kr = tile_rsrc(kb, ksb, t.key0, rows, dimb), Vr = tile_rsrc(vb, vsb, t.key0, rows, dimb);
 #pragma unroll
     for (int i = 0; i < NL; ++i) rk[i] = buffer_load_b128(Kr, ok[i]);
 #pragma unroll
     for (int i = 0; i < NL; ++i) rv[i] = buffer_load_b128(Vr, ov[i]);
   };
-  const auto store = [&](int stage) {
-    char* base = smem + stage * STAGE;
+  const auto store = [&](int slot) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
-      *reinterpret_cast<uint4*>(base + r * R::K_ROWB + col * 16) = rk[i];
-      *reinterpret_cast<uint4*>(base + VOFF + r * R::V_ROWB + col * 16) = rv[i];
+      if (NP % 256 == 0 || c < NP) {
+        *reinterpret_cast<uint4*>(smem + slot * (KB + VB) + r * R::K_ROWB + col * 16) = rk[i];
+        *reinterpret_cast<uint4*>(smem + slot * (KB + VB) + KB + r * R::V_ROWB + col * 16) = rv[i];
+      }
     }
   };
-
-  if (t0 < t1) {
-    load(t0);
-    store(0);
-  }
-  __syncthreads();
-  for (int t = t0; t < t1; ++t) {
-    if (t + 1 < t1) load(t + 1);
-    int key0, kend;
-    tile(t, key0, kend);
-    const bool unseen = key0 >= whi1 || (min(key0 + KT, kend) <= wlo0 && key0 >= a.sinks);
-    if (!idle && !unseen) {
-      const bool border = !(key0 + KT <= min(whi0, kend) && (key0 >= wlo1 || key0 + KT <= a.sinks));
-      const char* base = smem + ((t - t0) & 1) * STAGE;
-      const char* sk = base + ql * R::K_ROWB + half * 16;
-      f32x16 s[NB];
+  const float c = a.scale_log2;
+  const auto work = [&](const Tiles& t, int slot) {
+    bool any = false;
+    bool seen[RT];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
-#pragma unroll
-        for (int k = 0; k < R::NKS; ++k) Win<T>::mma(s[nb], *reinterpret_cast<const uint4*>(sk + nb * 32 * R::K_ROWB + k * 32), st.fq[k]);
-      }
-      st.softmax(s, key0, kend, half, border, a);
-      st.product(s, base + VOFF, lane);
+    for (int x = 0; x < RT; ++x) {  // by any row of the group (wave-uniform)
+      seen[x] = t.key0 < whi1[x] && (min(t.key0 + KT, t.kend) > wlo0[x] || t.key0 < a.sinks);
+      any = any || seen[x];
     }
-    if (t + 1 < t1) store((t + 1 - t0) & 1);
+    if (!any) return;
+    const char* sk = smem + slot * (KB + VB) + ql * R::K_ROWB + half * 16;
+    const char* sv = smem + slot * (KB + VB) + KB;
+    f32x16 s[RT][NB];
+#pragma unroll
+    for (int x = 0; x < RT; ++x)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[x][nb][r] = 0.f;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int k = 0; k < R::NKS; ++k) {
+        const uint4 fk = *reinterpret_cast<const uint4*>(sk + nb * 32 * R::K_ROWB + k * 32);
+#pragma unroll
+        for (int x = 0; x < RT; ++x) Win<T>::mma(s[x][nb], fk, st[x].fq[k]);
+      }
+#pragma unroll
+    for (int x = 0; x < RT; ++x) {
+      st[x].mask(s[x], t.key0, t.kend, half, t.key0 + KT > min(whi0[x], t.kend), t.key0 < wlo1[x] && t.key0 + KT > a.sinks, a.sinks);
+      st[x].raise(s[x], c);
+    }
+#pragma unroll
+    for (int g = 0; g < NB * R::PHASES_PER_BLOCK; ++g) {
+      typename R::VFrag f;
+      st[0].read_v(f, g, sv, lane);
+#pragma unroll
+      for (int x = 0; x < RT; ++x) st[x].weigh(s[x], g, c, f);
+    }
+  };
+  if (t0 < t1) {
+    Tiles at{t0 < na ? t0 * KT : bb + (t0 - na) * KT, t0 < na ? ea : khigh, bb, khigh}, ahead = at;
+    load(at);
+    store(0);
     __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+      const int slot = (t - t0) & 1;
+      ahead.next<KT>();
+      if (t + 1 < t1) load(ahead);
+      work(at, slot);
+      if (t + 1 < t1) store(slot ^ 1);
+      __syncthreads();
+      at = ahead;
+    }
   }
 
-  const float l = both_halves_sum(st.l);
-  if (!live) return;
-  if (a.nsplit > 1) {
-    const int64_t part = (((int64_t)b * a.heads + head) * a.tq + tok) * a.nsplit + ks;
-    float* po = a.part_o + part * a.dim;
+#pragma unroll
+  for (int x = 0; x < RT; ++x) {
+    const float l = both_halves_sum(st[x].l);
+    if (tok[x] >= nq) continue;
+    if (a.nsplit > 1) {
+      const int64_t part = (((int64_t)b * a.heads + head[x]) * a.tq + tok[x]) * a.nsplit + ks;
+      float* po = a.part_o + part * a.dim;
+#pragma unroll
+      for (int d = 0; d < R::ND; ++d)
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          const int col = d * 32 + 8 * c4 + 4 * half;
+          if (col < a.dim)
+            *reinterpret_cast<float4*>(po + col) = make_float4(st[x].o[d][4 * c4], st[x].o[d][4 * c4 + 1], st[x].o[d][4 * c4 + 2], st[x].o[d][4 * c4 + 3]);
+        }
+      if (half == 0) {
+        a.part_ml[part * 2] = st[x].m == -INFINITY ? -INFINITY : st[x].mc;
+        a.part_ml[part * 2 + 1] = l;
+      }
+      continue;
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    T* op = static_cast<T*>(a.out) + b * a.out_stride[0] + tok[x] * a.out_stride[1] + head[x] * a.out_stride[2];
 #pragma unroll
     for (int d = 0; d < R::ND; ++d)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int col = d * 32 + 8 * c + 4 * half;
-        if (col < a.dim) *reinterpret_cast<float4*>(po + col) = make_float4(st.o[d][4 * c], st.o[d][4 * c + 1], st.o[d][4 * c + 2], st.o[d][4 * c + 3]);
+      for (int c4 = 0; c4 < 4; ++c4) {
+        const int col = d * 32 + 8 * c4 + 4 * half;
+        if (col < a.dim) store4(op + col, st[x].o[d][4 * c4] * inv, st[x].o[d][4 * c4 + 1] * inv, st[x].o[d][4 * c4 + 2] * inv, st[x].o[d][4 * c4 + 3] * inv);
       }
-    if (half == 0) {
-      a.part_ml[part * 2] = st.m == -INFINITY ? -INFINITY : st.mc;
-      a.part_ml[part * 2 + 1] = l;
-    }
-    return;
   }
-  const float inv = l > 0.f ? 1.0f / l : 0.f;
-  T* op = static_cast<T*>(a.out) + b * a.out_stride[0] + tok * a.out_stride[1] + head * a.out_stride[2];
-#pragma unroll
-  for (int d = 0; d < R::ND; ++d)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int col = d * 32 + 8 * c + 4 * half;
-      if (col < a.dim) store4(op + col, st.o[d][4 * c] * inv, st.o[d][4 * c + 1] * inv, st.o[d][4 * c + 2] * inv, st.o[d][4 * c + 3] * inv);
-    }
 }
 
 // ---- few rows: one 32-row group, the waves along the keys ----------------------------------------------------------------------------------------
@@ -459,10 +529,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
       *reinterpret_cast<uint4*>(sv + r * R::V_ROWB + col * 16) = rv[i];
     }
     if (t + NW < t1) load_v(t + NW);
-    const bool border = !(key0 + KT <= min(high0, kend) && (key0 >= low1 || key0 + KT <= a.sinks));
-    st.softmax(s, key0, kend, half, border, a);
+    st.mask(s, key0, kend, half, key0 + KT > min(high0, kend), key0 < low1 && key0 + KT > a.sinks, a.sinks);
+    st.raise(s, a.scale_log2);
     wave_lds_sync();
-    st.product(s, sv, lane);
+#pragma unroll
+    for (int g = 0; g < R::PHASES_PER_BLOCK; ++g) {
+      typename R::VFrag f;
+      st.read_v(f, g, sv, lane);
+      st.weigh(s, g, a.scale_log2, f);
+    }
   }
 
   // the waves' parts: common reference, then 32 columns at a time through LDS, summed in the waves' order

@@ -126,6 +126,9 @@ ATTENTION = {
     "chunk_longer_than_keys": (1, 12, 7, 2, 2, 64, "fp16", 3, 0, 1, "end", None, None),
     "both_sides": (1, 150, 150, 2, 2, 64, "fp16", 20, 30, 40, "start", None, None),
     "both_sides_bf16_128": (1, 130, 130, 2, 1, 128, "bf16", 33, 17, 3, "start", None, None),
+    "both_sides_96": (1, 70, 70, 2, 1, 96, "fp16", 12, 30, 3, "start", None, None),
+    "both_sides_40": (1, 70, 90, 3, 1, 40, "bf16", 50, 3, 20, "start", None, None),
+    "fp32_96": (1, 50, 90, 3, 1, 96, "fp32", 50, 3, 20, "end", None, None),
     "causal": (1, 97, 97, 2, 2, 64, "bf16", -1, 0, 0, "start", None, None),
     "full": (1, 70, 70, 2, 2, 64, "fp16", -1, -1, 0, "start", None, None),
     "fp32_both_sides": (1, 140, 140, 2, 2, 64, "fp32", 25, 25, 30, "start", None, None),

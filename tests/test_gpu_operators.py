@@ -79,6 +79,8 @@ def test_window_attention(name):
     (5, 1, 4000, 16, 4, 128, "fp16", 2047, 0, 4, "end", [4000, 1, 0, 2500, 333], None),
     (2, 4, 9000, 8, 1, 64, "bf16", -1, 0, 0, "end", [9000, 5000], [4, 1]),
     (1, 2, 2500, 4, 4, 128, "fp32", 2000, 0, 100, "end", None, None),
+    (16, 330, 330, 32, 32, 64, "fp16", 60, 40, 75, "start", [330 - 20 * i for i in range(16)], None),
+    (9, 300, 700, 64, 64, 64, "bf16", 90, 0, 5, "end", None, [300 - 35 * i for i in range(9)]),
     (2, 1, 300, 40, 1, 96, "fp16", 250, 0, 9, "end", None, None),
 ], ids=lambda c: "-".join(map(str, c[:7])))
 def test_window_attention_larger(case):
