@@ -15,7 +15,7 @@ Plan plan_of(const f5hip_window_attention_args& a) {
   const int64_t rows = (int64_t)a.q_tokens * (a.heads / a.kv_heads), heads = (int64_t)a.batch * a.kv_heads;
   Plan p;
   p.few = rows <= 32;
-  p.groups = !p.few && a.dtype != F5HIP_T_FP32 && a.head_dim <= 64 && heads * ((rows + 255) / 256) >= 512 ? 2 : 1;
+  p.groups = !p.few && a.dtype != F5HIP_T_FP32 && a.head_dim <= 64 && heads * ((rows + 255) / 256) >= 512000 ? 2 : 1;
   const int per = p.few ? 32 : 128 * p.groups;
   p.nblk = (int)((rows + per - 1) / per);
   // the most keys a row block can see

@@ -249,6 +249,12 @@ __device__ __forceinline__ int xcd_order(int b, int n) {
   const int q = n >> 3, r = n & 7, x = b & 7;
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (b >> 3);
 }
+// ... and deal the (sequence, key head) units to those ranges in turn: place i of the order is unit 0, 8, 16 ..., 1, 9 ...  Neighbouring units are heads of
+// one sequence, so sequences of different lengths would otherwise load the XCDs differently.
+__device__ __forceinline__ int spread_units(int i, int n) {
+  const int q = n >> 3, r = n & 7, big = r * (q + 1);
+  return i < big ? (i % (q + 1)) * 8 + i / (q + 1) : ((i - big) % q) * 8 + r + (i - big) / q;
+}
 
 // ---- many rows: 4 waves x RT groups of 32 rows, K and V tiles shared through LDS, two stages ------------------------------------------------------
 // The tiles of a row block in order: keys [0, ea), then [bb, high).  One cursor walks them for the loads, one for the work; advancing costs a few scalar
@@ -273,7 +279,7 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
   int L = xcd_order((int)blockIdx.x, a.nwg);
   const int ks = L % a.nsplit;
   L /= a.nsplit;
-  const int blk = L % a.nblk, bh = L / a.nblk, b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
+  const int blk = L % a.nblk, bh = spread_units(L / a.nblk, a.batch * a.kv_heads), b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
   const int n = a.kv_len ? max(0, min(a.kv_len[b], a.tk)) : a.tk, nq = a.q_len ? max(0, min(a.q_len[b], a.tq)) : a.tq;
   const int first = blk * ROWS / a.group;
   if (first >= nq) return;  // (the whole workgroup: no barrier has been reached)
@@ -450,7 +456,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
   int L = xcd_order((int)blockIdx.x, a.nwg);
   const int ks = L % a.nsplit;
   L /= a.nsplit;
-  const int blk = L % a.nblk, bh = L / a.nblk, b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
+  const int blk = L % a.nblk, bh = spread_units(L / a.nblk, a.batch * a.kv_heads), b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
   const int n = a.kv_len ? max(0, min(a.kv_len[b], a.tk)) : a.tk, nq = a.q_len ? max(0, min(a.q_len[b], a.tq)) : a.tq;
   const int first = blk * 32 / a.group;
   if (first >= nq) return;  // (the whole workgroup)
