@@ -369,26 +369,41 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[x][nb][r] = 0.f;
+    // Operands are read from LDS one step ahead of the matrix instructions that take them — four K pieces, or the V pieces of a phase — and the scheduling
+    // barriers keep the compiler from sinking the reads back to their uses (a wave then sits out an LDS round trip at each).
+    constexpr int NQ = NB * R::NKS / 4, PH = NB * R::PHASES_PER_BLOCK;
+    uint4 fk[2][4];
+    const auto read_k = [&](auto C) {
+      constexpr int q = decltype(C)::value;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+      for (int i = 0; i < 4; ++i) fk[q & 1][i] = *reinterpret_cast<const uint4*>(sk + (4 * q + i) / R::NKS * 32 * R::K_ROWB + (4 * q + i) % R::NKS * 32);
+    };
+    typename R::VFrag fv[2];
+    read_k(std::integral_constant<int, 0>{});
+    static_for<NQ>([&](auto Q) {
+      constexpr int q = decltype(Q)::value;
+      if constexpr (q + 1 < NQ) read_k(std::integral_constant<int, q + 1>{});
+      else st[0].read_v(fv[0], 0, sv, lane);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < R::NKS; ++k) {
-        const uint4 fk = *reinterpret_cast<const uint4*>(sk + nb * 32 * R::K_ROWB + k * 32);
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int x = 0; x < RT; ++x) Win<T>::mma(s[x][nb], fk, st[x].fq[k]);
-      }
+        for (int x = 0; x < RT; ++x) Win<T>::mma(s[x][(4 * q + i) / R::NKS], fk[q & 1][i], st[x].fq[(4 * q + i) % R::NKS]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
 #pragma unroll
     for (int x = 0; x < RT; ++x) {
       st[x].mask(s[x], t.key0, t.kend, half, t.key0 + KT > min(whi0[x], t.kend), t.key0 < wlo1[x] && t.key0 + KT > a.sinks, a.sinks);
       st[x].raise(s[x], c);
     }
+    static_for<PH>([&](auto G) {
+      constexpr int g = decltype(G)::value;
+      if constexpr (g + 1 < PH) st[0].read_v(fv[(g + 1) & 1], g + 1, sv, lane);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int g = 0; g < NB * R::PHASES_PER_BLOCK; ++g) {
-      typename R::VFrag f;
-      st[0].read_v(f, g, sv, lane);
-#pragma unroll
-      for (int x = 0; x < RT; ++x) st[x].weigh(s[x], g, c, f);
-    }
+      for (int x = 0; x < RT; ++x) st[x].weigh(s[x], g, c, fv[g & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
   if (t0 < t1) {
     Tiles at{t0 < na ? t0 * KT : bb + (t0 - na) * KT, t0 < na ? ea : khigh, bb, khigh}, ahead = at;
