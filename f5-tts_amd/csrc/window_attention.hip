@@ -4,25 +4,32 @@
 #include "window_attention_kernel.h"
 
 namespace {
-// Few rows (window_few_kernel: waves along the keys) up to 32 rows of a key head, many (window_rows_kernel: waves along the rows) above.  The keys are cut
-// into ranges where the row blocks alone leave CUs idle; both kernels then leave partial results that window_join_kernel merges.
+// Few rows (window_few_kernel: waves along the keys) up to 32 rows of a key head, many (window_rows_kernel: waves along the rows) above.
+// Many rows: 128 rows a workgroup, or, up to 64 columns and where that makes fewer than four workgroups a CU, 64 rows whose two waves share the keys
+// (KG = 2).  Measured on an MI355X: 2 x 1406 frames, 16 heads of 64, 1026 keys seen (352 blocks of 128 rows) 24 us with 64 rows, 33 us with 128; 16 ragged
+// utterances of 12 heads (1920 blocks) 59 and 48 us; 2 x 8192 frames (2048 blocks) 170 and 148 us; with 128 columns (6 chunks of 200 tokens, 32 heads on 8,
+// 336 blocks) 81 and 75 us: there the tiles are twice as large, and loading them for 64 rows costs more than the better balance brings.
+// Ranges of keys over workgroups, joined by window_join_kernel, where the blocks alone leave CUs without two workgroups: at least 256 keys each (few
+// rows: 512, two tiles a wave).  More ranges balance better and lose it to the partial results' way out and back (the chunks in two ranges 75 us, three 81,
+// four 89).
 struct Plan {
   bool few;
-  int groups;  // many rows: 32-row groups of a wave
+  int ranges;  // many rows: key ranges of a workgroup (window_rows_kernel's KG)
   int nblk, nsplit;
 };
 Plan plan_of(const f5hip_window_attention_args& a) {
-  const int64_t rows = (int64_t)a.q_tokens * (a.heads / a.kv_heads), heads = (int64_t)a.batch * a.kv_heads;
-  Plan p;
+  const int group = a.heads / a.kv_heads;
+  const int64_t rows = (int64_t)a.q_tokens * group, units = (int64_t)a.batch * a.kv_heads;
+  Plan p{};
   p.few = rows <= 32;
-  p.groups = !p.few && a.dtype != F5HIP_T_FP32 && a.head_dim <= 64 && heads * ((rows + 255) / 256) >= 512000 ? 2 : 1;
-  const int per = p.few ? 32 : 128 * p.groups;
+  p.ranges = a.head_dim <= 64 && units * ((rows + 127) / 128) < 1024 ? 2 : 1;
+  const int per = p.few ? 32 : 128 / p.ranges;
   p.nblk = (int)((rows + per - 1) / per);
-  // the most keys a row block can see
-  const int64_t tokens = std::min<int64_t>(a.q_tokens, per / (a.heads / a.kv_heads) + 2);
+  // the most keys that a block's queries can see
   int64_t keys = a.kv_tokens;
-  if (a.window_left >= 0 && a.window_right >= 0) keys = std::min<int64_t>(keys, (int64_t)a.window_left + a.window_right + tokens + std::min(a.sinks, a.kv_tokens));
-  const int64_t blocks = heads * p.nblk, want = (512 + blocks - 1) / blocks, most = p.few ? keys / 512 : keys / 256;
+  if (a.window_left >= 0 && a.window_right >= 0)
+    keys = std::min<int64_t>(keys, (int64_t)a.window_left + a.window_right + std::min<int64_t>(a.q_tokens, per / group + 2) + std::min(a.sinks, a.kv_tokens));
+  const int64_t blocks = units * p.nblk, want = (512 + blocks - 1) / blocks, most = keys / (p.few ? 512 : 256);
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, most), 64));
   return p;
 }
@@ -33,8 +40,8 @@ hipError_t launch(const WindowArgs& w, const Plan& p, hipStream_t s) {
   const auto go = [&](auto DP) {
     constexpr int dp = decltype(DP)::value;
     if (p.few) hipLaunchKernelGGL((window_few_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(64 * FEW_WAVES<T>), 0, s, w);
-    else if (p.groups == 1) hipLaunchKernelGGL((window_rows_kernel<T, dp, 1>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
-    else if constexpr (sizeof(T) == 2 && dp == 64) hipLaunchKernelGGL((window_rows_kernel<T, dp, 2>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
+    else if (p.ranges == 1) hipLaunchKernelGGL((window_rows_kernel<T, dp, 1>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
+    else hipLaunchKernelGGL((window_rows_kernel<T, dp, 2>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
   };
   if (w.dim <= 64) go(std::integral_constant<int, 64>{});
   else if (w.dim <= 96) go(std::integral_constant<int, 96>{});

@@ -10,9 +10,11 @@
 // half-wave exchange; those registers are, as they stand, the other operand of O^T += V^T P^T (the contraction runs over keys in the
 // accumulator's own order), so P never moves.  V^T fragments come from row-major V tiles by the transposing LDS read (16-bit types) or as
 // single floats.
-// Softmax.  exp2(c s - c m) with c = scale log2 e > 0 (a negative scale's sign is folded into q).  m is a reference, not the exact maximum: it
-// is raised (and O, l rescaled) only where a tile exceeds it by more than 8 in the exponent.  fp16 weights are held times 2^7, up to 2^15: those
-// as small as 2^-21 of the row's largest are then normal numbers, rounded relative to themselves.
+// Softmax.  exp2(c s - c m) with c = scale log2 e > 0 (a negative scale's sign is folded into q).  m is a reference, not the running maximum, and no
+// maximum is taken on the common path: the weights of a tile are summed anyway, and only where a lane's sum passes 2^15 — the reference is some 2^8 too
+// low, or none has been set — is the tile's maximum taken, O and l rescaled, and the tile's weights computed again.  The reference is set so that the
+// row's largest weight is 2^BIAS: in fp16 2^7, so that weights up to 2^15 are finite and those as small as 2^-21 of the largest are normal numbers,
+// rounded relative to themselves.
 #pragma once
 #include <math.h>
 
@@ -122,8 +124,9 @@ struct Rows {
   static constexpr int EB = sizeof(T), ND = DP / 32, NKS = DP * EB / 32;
   static constexpr int K_ROWB = DP * EB + 16;                              // 32 rows read 16 bytes each without conflicts
   static constexpr int V_ROWB = EB == 4 ? DP * 4 + 32 : (DP == 64 ? 192 : 320);  // 16 bit: 4 rows start 64 bytes apart in the 256-byte bank row
+  static constexpr float UNSET = -1e30f, LIMIT = 32768.0f;
   f32x16 o[ND];
-  float m, mc, l;  // reference maximum (raw score; -inf: nothing seen), c m - BIAS (0 then), this lane's share of the row sum
+  float mc, l;  // c m - BIAS (UNSET: no key seen, any score passes the limit), this lane's share of the row sum
   int lo, hi;      // the lane's row: its window
   uint4 fq[NKS];
 
@@ -132,8 +135,7 @@ struct Rows {
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    m = -INFINITY;
-    mc = 0.f;
+    mc = UNSET;
     l = 0.f;
   }
 
@@ -159,7 +161,7 @@ struct Rows {
     }
   }
 
-  // the reference maximum, raised (and O, l rescaled) where the tile goes far above it
+  // the reference raised to the tile's maximum (O, l rescaled); rows that see nothing keep theirs
   template <int NB>
   __device__ __forceinline__ void raise(const f32x16 (&s)[NB], float c) {
     float mx = s[0][0];
@@ -167,18 +169,13 @@ struct Rows {
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
-    mx = both_halves_max(mx);
-    if (f5_wave_any(fmaf(mx, c, -mc) > 8.0f + Win<T>::BIAS || (m == -INFINITY && mx > -INFINITY))) {
-      const float mn = fmaxf(m, mx), mnc = mn == -INFINITY ? 0.f : fmaf(mn, c, -Win<T>::BIAS);
-      const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - mnc);
+    const float to = fmaxf(mc, fmaf(both_halves_max(mx), c, -Win<T>::BIAS)), al = __builtin_amdgcn_exp2f(mc - to);
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[d][r] *= al;
-      l *= al;
-      m = mn;
-      mc = mnc;
-    }
+      for (int r = 0; r < 16; ++r) o[d][r] *= al;
+    l *= al;
+    mc = to;
   }
 
   // A tile is worked through in phases, PHASES_PER_BLOCK for each 32 keys: 16 keys a phase in 16-bit types (the lane's are 16 g + 4 half + 0..3
@@ -205,35 +202,57 @@ struct Rows {
       }
     }
   }
-  // the weights of phase g's keys, and O^T += V^T P^T over them
+  // the weights of a tile's keys, as the second product takes them, and the row sum; the reference raised where it has to be
   template <int NB>
-  __device__ __forceinline__ void weigh(const f32x16 (&s)[NB], int g, float c, const VFrag& f) {
-    if constexpr (EB == 2) {
-      uint32_t p[4];
+  struct Weights {
+    uint32_t p[NB * (EB == 2 ? 8 : 16)];  // 16-bit types: pairs; fp32: one each, in the scores' order
+  };
+  template <int NB>
+  __device__ __forceinline__ float weights_once(const f32x16 (&s)[NB], Weights<NB>& w, float c) const {
+    float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * e], c, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + 2 * e + 1], c, -mc));
-        p[e] = Win<T>::pack(x, y);
-        l = Win<T>::add2(p[e], l);  // the sum is that of the rounded weights: numerator and denominator see the same ones
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[n][r + 1], c, -mc));
+        if constexpr (EB == 2) {
+          const uint32_t p = Win<T>::pack(x, y);
+          w.p[n * 8 + r / 2] = p;
+          sum = Win<T>::add2(p, sum);  // of the rounded weights: numerator and denominator see the same ones
+        } else {
+          w.p[n * 16 + r] = __builtin_bit_cast(uint32_t, x);
+          w.p[n * 16 + r + 1] = __builtin_bit_cast(uint32_t, y);
+          sum += x + y;
+        }
       }
-      const uint4 fp = make_uint4(p[0], p[1], p[2], p[3]);
+    return sum;
+  }
+  template <int NB>
+  __device__ __forceinline__ void weigh(const f32x16 (&s)[NB], Weights<NB>& w, float c) {
+    float sum = weights_once(s, w, c);
+    if (f5_wave_any(sum > LIMIT)) {
+      raise(s, c);
+      sum = weights_once(s, w, c);
+    }
+    l += sum;
+  }
+  // O^T += V^T P^T over phase g's keys
+  template <int NB>
+  __device__ __forceinline__ void product(const Weights<NB>& w, int g, const VFrag& f) {
+    const uint4 p = make_uint4(w.p[4 * g], w.p[4 * g + 1], w.p[4 * g + 2], w.p[4 * g + 3]);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) Win<T>::mma(o[d], f.v[d], fp);
-    } else {
-      float w[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[e] = __builtin_amdgcn_exp2f(fmaf(s[g >> 2][4 * (g & 3) + e], c, -mc));
-        l += w[e];
-      }
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const uint32_t v[4] = {f.v[d].x, f.v[d].y, f.v[d].z, f.v[d].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, v[e]), w[e], o[d], 0, 0, 0);
+    for (int d = 0; d < ND; ++d) {
+      if constexpr (EB == 2) {
+        Win<T>::mma(o[d], f.v[d], p);
+      } else {
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, f.v[d].x), __builtin_bit_cast(float, p.x), o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, f.v[d].y), __builtin_bit_cast(float, p.y), o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, f.v[d].z), __builtin_bit_cast(float, p.z), o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, f.v[d].w), __builtin_bit_cast(float, p.w), o[d], 0, 0, 0);
       }
     }
   }
+  __device__ __forceinline__ float reference() const { return mc == UNSET ? -INFINITY : mc; }
 };
 
 // four neighbouring columns of an output row
@@ -256,7 +275,9 @@ __device__ __forceinline__ int spread_units(int i, int n) {
   return i < big ? (i % (q + 1)) * 8 + i / (q + 1) : ((i - big) % q) * 8 + r + (i - big) / q;
 }
 
-// ---- many rows: 4 waves x RT groups of 32 rows, K and V tiles shared through LDS, two stages ------------------------------------------------------
+// ---- many rows: K and V tiles of 64 keys shared through LDS, two stages ------------------------------------------------------------------------------
+// Four waves: 4 / KG groups of 32 rows x KG ranges of keys.  KG = 1: 128 rows a workgroup, a wave takes whole tiles.  KG = 2: 64 rows, a wave takes one half
+// of every tile and the two halves' results meet in LDS at the end — twice the workgroups, each half as long, where row blocks alone load the CUs unevenly.
 // The tiles of a row block in order: keys [0, ea), then [bb, high).  One cursor walks them for the loads, one for the work; advancing costs a few scalar
 // instructions where indexing by a tile number took ninety.
 struct Tiles {
@@ -269,12 +290,12 @@ struct Tiles {
   }
 };
 
-template <typename T, int DP, int RT>
-__global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
+template <typename T, int DP, int KG>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window_rows_kernel(WindowArgs a) {
   using R = Rows<T, DP>;
-  constexpr int KT = sizeof(T) == 2 ? 64 : 32, NB = KT / 32, EB = R::EB, CPR = DP * EB / 16, NP = KT * CPR, NL = (NP + 255) / 256, ROWS = 128 * RT;
-  constexpr int KB = KT * R::K_ROWB, VB = KT * R::V_ROWB;
-  __shared__ __attribute__((aligned(16))) char smem[2 * (KB + VB)];
+  constexpr int KT = sizeof(T) == 2 || KG == 2 ? 64 : 32, NB = KT / 32 / KG, EB = R::EB, CPR = DP * EB / 16, NP = KT * CPR, NL = (NP + 255) / 256, ROWS = 128 / KG;
+  constexpr int KB = KT * R::K_ROWB, VB = KT * R::V_ROWB, STAGES = sizeof(T) == 4 && DP > 64 && KG == 2 ? 1 : 2;
+  __shared__ __attribute__((aligned(16))) char smem[STAGES * (KB + VB)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, ql = lane & 31;
   int L = xcd_order((int)blockIdx.x, a.nwg);
   const int ks = L % a.nsplit;
@@ -291,32 +312,23 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
   const int na = (ea + KT - 1) / KT, nt = na + (khigh - bb + KT - 1) / KT;
   const int t0 = (int)((int64_t)ks * nt / a.nsplit), t1 = (int)((int64_t)(ks + 1) * nt / a.nsplit);
 
-  // the wave's rows: RT groups of 32, a lane's row in each
-  R st[RT];
-  const T* qp[RT];
-  int tok[RT], head[RT], whi0[RT], whi1[RT], wlo0[RT], wlo1[RT];
+  // the wave's rows, the lane's row
+  const int r0 = blk * ROWS + wave / KG * 32, kg = wave % KG, row = r0 + ql, tok = row / a.group, head = kvh * a.group + (row - tok * a.group);
+  const bool live = tok < nq;
+  const int wfirst = r0 / a.group, wlast = min(nq - 1, (r0 + 31) / a.group);
+  // the tightest and widest borders of the wave's rows; no row at all: nothing is seen
+  const int whi0 = sp.high(p0 + wfirst), whi1 = wfirst < nq ? sp.high(p0 + wlast) : 0, wlo0 = sp.low(p0 + wfirst), wlo1 = sp.low(p0 + wlast);
+  R st;
+  st.reset();
+  st.lo = sp.low(p0 + tok);
+  st.hi = live ? sp.high(p0 + tok) : 0;
+  const T* qp = static_cast<const T*>(a.q) + b * a.q_stride[0] + tok * a.q_stride[1] + head * a.q_stride[2];
 #pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    const int r0 = blk * ROWS + (wave * RT + x) * 32, row = r0 + ql;
-    tok[x] = row / a.group;
-    head[x] = kvh * a.group + (row - tok[x] * a.group);
-    const int wfirst = r0 / a.group, wlast = min(nq - 1, (r0 + 31) / a.group);
-    // the tightest and widest borders of the group's rows; no row at all: nothing is seen
-    whi0[x] = sp.high(p0 + wfirst);
-    whi1[x] = wfirst < nq ? sp.high(p0 + wlast) : 0;
-    wlo0[x] = sp.low(p0 + wfirst);
-    wlo1[x] = sp.low(p0 + wlast);
-    st[x].reset();
-    st[x].lo = sp.low(p0 + tok[x]);
-    st[x].hi = tok[x] < nq ? sp.high(p0 + tok[x]) : 0;
-    qp[x] = static_cast<const T*>(a.q) + b * a.q_stride[0] + tok[x] * a.q_stride[1] + head[x] * a.q_stride[2];
-#pragma unroll
-    for (int k = 0; k < R::NKS; ++k) {
-      const int col = (k * 32 + half * 16) / EB;
-      uint4 u = tok[x] < nq && col < a.dim ? *reinterpret_cast<const uint4*>(qp[x] + col) : make_uint4(0, 0, 0, 0);
-      u.x ^= a.negate; u.y ^= a.negate; u.z ^= a.negate; u.w ^= a.negate;
-      st[x].fq[k] = u;
-    }
+  for (int k = 0; k < R::NKS; ++k) {
+    const int col = (k * 32 + half * 16) / EB;
+    uint4 u = live && col < a.dim ? *reinterpret_cast<const uint4*>(qp + col) : make_uint4(0, 0, 0, 0);
+    u.x ^= a.negate; u.y ^= a.negate; u.z ^= a.negate; u.w ^= a.negate;
+    st.fq[k] = u;
   }
 
   const int64_t ksb = a.k_stride[1] * EB, vsb = a.v_stride[1] * EB;
@@ -352,56 +364,44 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
   };
   const float c = a.scale_log2;
   const auto work = [&](const Tiles& t, int slot) {
-    bool any = false;
-    bool seen[RT];
+    const int key0 = t.key0 + kg * 32 * NB;  // the wave's keys of the tile
+    if (key0 >= min(whi1, t.kend) || (min(key0 + 32 * NB, t.kend) <= wlo0 && key0 >= a.sinks)) return;  // none of its rows sees one (wave-uniform)
+    const char* sk = smem + slot * (KB + VB) + (kg * 32 * NB + ql) * R::K_ROWB + half * 16;
+    const char* sv = smem + slot * (KB + VB) + KB + kg * 32 * NB * R::V_ROWB;
+    f32x16 s[NB];
 #pragma unroll
-    for (int x = 0; x < RT; ++x) {  // by any row of the group (wave-uniform)
-      seen[x] = t.key0 < whi1[x] && (min(t.key0 + KT, t.kend) > wlo0[x] || t.key0 < a.sinks);
-      any = any || seen[x];
-    }
-    if (!any) return;
-    const char* sk = smem + slot * (KB + VB) + ql * R::K_ROWB + half * 16;
-    const char* sv = smem + slot * (KB + VB) + KB;
-    f32x16 s[RT][NB];
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int x = 0; x < RT; ++x)
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[x][nb][r] = 0.f;
-    // Operands are read from LDS one step ahead of the matrix instructions that take them — four K pieces, or the V pieces of a phase — and the scheduling
+      for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
+    // Operands are read from LDS one step ahead of the matrix instructions that take them — four (three) K pieces, or the V pieces of a phase — and the scheduling
     // barriers keep the compiler from sinking the reads back to their uses (a wave then sits out an LDS round trip at each).
-    constexpr int NQ = NB * R::NKS / 4, PH = NB * R::PHASES_PER_BLOCK;
-    uint4 fk[2][4];
+    constexpr int QS = NB * R::NKS % 4 == 0 ? 4 : 3, NQ = NB * R::NKS / QS, PH = NB * R::PHASES_PER_BLOCK;
+    static_assert(NB * R::NKS % QS == 0, "whole steps of K pieces");
+    uint4 fk[2][QS];
     const auto read_k = [&](auto C) {
       constexpr int q = decltype(C)::value;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) fk[q & 1][i] = *reinterpret_cast<const uint4*>(sk + (4 * q + i) / R::NKS * 32 * R::K_ROWB + (4 * q + i) % R::NKS * 32);
+      for (int i = 0; i < QS; ++i) fk[q & 1][i] = *reinterpret_cast<const uint4*>(sk + (QS * q + i) / R::NKS * 32 * R::K_ROWB + (QS * q + i) % R::NKS * 32);
     };
     typename R::VFrag fv[2];
     read_k(std::integral_constant<int, 0>{});
     static_for<NQ>([&](auto Q) {
       constexpr int q = decltype(Q)::value;
       if constexpr (q + 1 < NQ) read_k(std::integral_constant<int, q + 1>{});
-      else st[0].read_v(fv[0], 0, sv, lane);
+      else st.read_v(fv[0], 0, sv, lane);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int x = 0; x < RT; ++x) Win<T>::mma(s[x][(4 * q + i) / R::NKS], fk[q & 1][i], st[x].fq[(4 * q + i) % R::NKS]);
+      for (int i = 0; i < QS; ++i) Win<T>::mma(s[(QS * q + i) / R::NKS], fk[q & 1][i], st.fq[(QS * q + i) % R::NKS]);
       __builtin_amdgcn_sched_barrier(0);
     });
-#pragma unroll
-    for (int x = 0; x < RT; ++x) {
-      st[x].mask(s[x], t.key0, t.kend, half, t.key0 + KT > min(whi0[x], t.kend), t.key0 < wlo1[x] && t.key0 + KT > a.sinks, a.sinks);
-      st[x].raise(s[x], c);
-    }
+    st.mask(s, key0, t.kend, half, key0 + 32 * NB > min(whi0, t.kend), key0 < wlo1 && key0 + 32 * NB > a.sinks, a.sinks);
+    typename R::template Weights<NB> w;
+    st.weigh(s, w, c);
     static_for<PH>([&](auto G) {
       constexpr int g = decltype(G)::value;
-      if constexpr (g + 1 < PH) st[0].read_v(fv[(g + 1) & 1], g + 1, sv, lane);
+      if constexpr (g + 1 < PH) st.read_v(fv[(g + 1) & 1], g + 1, sv, lane);
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int x = 0; x < RT; ++x) st[x].weigh(s[x], g, c, fv[g & 1]);
+      st.product(w, g, fv[g & 1]);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
@@ -411,47 +411,67 @@ __global__ __launch_bounds__(256, 2) void window_rows_kernel(WindowArgs a) {
     store(0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
-      const int slot = (t - t0) & 1;
+      const int slot = STAGES == 2 ? (t - t0) & 1 : 0;
       ahead.next<KT>();
       if (t + 1 < t1) load(ahead);
       work(at, slot);
-      if (t + 1 < t1) store(slot ^ 1);
+      if constexpr (STAGES == 1) __syncthreads();  // every wave has read the one stage
+      if (t + 1 < t1) store(STAGES == 2 ? slot ^ 1 : 0);
       __syncthreads();
       at = ahead;
     }
   }
 
-#pragma unroll
-  for (int x = 0; x < RT; ++x) {
-    const float l = both_halves_sum(st[x].l);
-    if (tok[x] >= nq) continue;
-    if (a.nsplit > 1) {
-      const int64_t part = (((int64_t)b * a.heads + head[x]) * a.tq + tok[x]) * a.nsplit + ks;
-      float* po = a.part_o + part * a.dim;
+  float l = both_halves_sum(st.l), top = st.reference();
+  if constexpr (KG == 2) {  // the second half's result through LDS (its places have been read: the loop ended at a barrier), columns as the lanes hold them
+    constexpr int LANE_FLOATS = 16 * R::ND + 2;
+    static_assert(STAGES * (KB + VB) >= 2 * 64 * LANE_FLOATS * 4, "the halves meet in the tiles' place");
+    float* x = reinterpret_cast<float*>(smem) + wave / 2 * 64 * LANE_FLOATS + lane;
+    if (kg == 1) {
 #pragma unroll
       for (int d = 0; d < R::ND; ++d)
 #pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4) {
-          const int col = d * 32 + 8 * c4 + 4 * half;
-          if (col < a.dim)
-            *reinterpret_cast<float4*>(po + col) = make_float4(st[x].o[d][4 * c4], st[x].o[d][4 * c4 + 1], st[x].o[d][4 * c4 + 2], st[x].o[d][4 * c4 + 3]);
-        }
-      if (half == 0) {
-        a.part_ml[part * 2] = st[x].m == -INFINITY ? -INFINITY : st[x].mc;
-        a.part_ml[part * 2 + 1] = l;
-      }
-      continue;
+        for (int r = 0; r < 16; ++r) x[(d * 16 + r) * 64] = st.o[d][r];
+      x[16 * R::ND * 64] = top;
+      x[(16 * R::ND + 1) * 64] = l;
     }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-    T* op = static_cast<T*>(a.out) + b * a.out_stride[0] + tok[x] * a.out_stride[1] + head[x] * a.out_stride[2];
+    __syncthreads();
+    if (kg == 1) return;
+    const float top1 = x[16 * R::ND * 64], l1 = x[(16 * R::ND + 1) * 64], both = fmaxf(top, top1);
+    const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - both), f1 = top1 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top1 - both);
+#pragma unroll
+    for (int d = 0; d < R::ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.o[d][r] = st.o[d][r] * f0 + x[(d * 16 + r) * 64] * f1;
+    l = l * f0 + l1 * f1;
+    top = both;
+  }
+  if (!live) return;
+  if (a.nsplit > 1) {
+    const int64_t part = (((int64_t)b * a.heads + head) * a.tq + tok) * a.nsplit + ks;
+    float* po = a.part_o + part * a.dim;
 #pragma unroll
     for (int d = 0; d < R::ND; ++d)
 #pragma unroll
       for (int c4 = 0; c4 < 4; ++c4) {
         const int col = d * 32 + 8 * c4 + 4 * half;
-        if (col < a.dim) store4(op + col, st[x].o[d][4 * c4] * inv, st[x].o[d][4 * c4 + 1] * inv, st[x].o[d][4 * c4 + 2] * inv, st[x].o[d][4 * c4 + 3] * inv);
+        if (col < a.dim) *reinterpret_cast<float4*>(po + col) = make_float4(st.o[d][4 * c4], st.o[d][4 * c4 + 1], st.o[d][4 * c4 + 2], st.o[d][4 * c4 + 3]);
       }
+    if (half == 0) {
+      a.part_ml[part * 2] = top;
+      a.part_ml[part * 2 + 1] = l;
+    }
+    return;
   }
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  T* op = static_cast<T*>(a.out) + b * a.out_stride[0] + tok * a.out_stride[1] + head * a.out_stride[2];
+#pragma unroll
+  for (int d = 0; d < R::ND; ++d)
+#pragma unroll
+    for (int c4 = 0; c4 < 4; ++c4) {
+      const int col = d * 32 + 8 * c4 + 4 * half;
+      if (col < a.dim) store4(op + col, st.o[d][4 * c4] * inv, st.o[d][4 * c4 + 1] * inv, st.o[d][4 * c4 + 2] * inv, st.o[d][4 * c4 + 3] * inv);
+    }
 }
 
 // ---- few rows: one 32-row group, the waves along the keys ----------------------------------------------------------------------------------------
@@ -551,20 +571,21 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
     }
     if (t + NW < t1) load_v(t + NW);
     st.mask(s, key0, kend, half, key0 + KT > min(high0, kend), key0 < low1 && key0 + KT > a.sinks, a.sinks);
-    st.raise(s, a.scale_log2);
+    typename R::template Weights<1> w;
+    st.weigh(s, w, a.scale_log2);
     wave_lds_sync();
 #pragma unroll
     for (int g = 0; g < R::PHASES_PER_BLOCK; ++g) {
       typename R::VFrag f;
       st.read_v(f, g, sv, lane);
-      st.weigh(s, g, a.scale_log2, f);
+      st.product(w, g, f);
     }
   }
 
   // the waves' parts: common reference, then 32 columns at a time through LDS, summed in the waves' order
   const float l = both_halves_sum(st.l);
   if (half == 0) {
-    sml[wave][ql][0] = st.m == -INFINITY ? -INFINITY : st.mc;
+    sml[wave][ql][0] = st.reference();
     sml[wave][ql][1] = l;
   }
   __syncthreads();
