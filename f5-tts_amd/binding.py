@@ -17,6 +17,7 @@ BENCH_LIB_PATH = os.environ.get("F5HIP_BENCH_LIB") or os.path.join(_HERE, "csrc"
 
 ABI_VERSION = 10  # F5HIP_ABI_VERSION in include/f5hip.h
 PREC_FP32, PREC_FP16X3, PREC_FP16, PREC_FP16M = 0, 1, 2, 3
+ROPE_SCALINGS = {None: 0, "none": 0, "linear": 1, "ntk": 2, "yarn": 3}  # F5HIP_ROPE_*
 PRECISIONS = {"fp32": PREC_FP32, "fp16x3": PREC_FP16X3, "fp16": PREC_FP16, "fp16m": PREC_FP16M}
 
 
@@ -37,6 +38,11 @@ class BigVGANConfigC(C.Structure):
                 ("num_kernels", C.c_int32), ("resblock_kernel_sizes", C.c_int32 * 4), ("resblock_num_dilations", C.c_int32 * 4),
                 ("resblock_dilation_sizes", (C.c_int32 * 4) * 4), ("activation", C.c_int32), ("snake_logscale", C.c_int32),
                 ("use_tanh_at_final", C.c_int32), ("use_bias_at_final", C.c_int32)]
+
+
+class LongFormC(C.Structure):
+    _fields_ = [("window_left", C.c_int32), ("window_right", C.c_int32), ("sinks", C.c_int32), ("rope_scaling", C.c_int32),
+                ("rope_factor", C.c_double), ("rope_original_length", C.c_int64)]
 
 
 # every symbol include/f5hip.h declares: name -> (restype, argtypes)
@@ -67,6 +73,7 @@ SYMBOLS = {
                                     C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     "f5hip_reset_kernel_stats": (C.c_int, [_P]),
     "f5hip_attention_stats": (C.c_int, [_P, C.POINTER(C.c_double), C.c_int]),
+    "f5hip_set_long_form": (C.c_int, [_P, C.POINTER(LongFormC)]),
     "f5hip_rotary_frequencies": (C.c_int, [C.c_int, C.c_double, C.c_int, C.c_double, C.c_int64, C.c_double, C.c_double, _P, C.POINTER(C.c_double)]),
     "f5hip_rotary": (C.c_int, [_P, C.c_int, _P]),
     "f5hip_window_attention_workspace": (C.c_int64, [_P]),

@@ -7,6 +7,7 @@
 #include <cstring>
 
 #include "engine.h"
+#include "operators.h"
 
 namespace {
 
@@ -415,6 +416,22 @@ float attn_qscale(int dh, bool exact_attn) { return (exact_attn ? 1.0f : 1.44269
 // FP16M: fp16x3 everywhere except the four block GEMMs of the DiT backbone, which read MX lines when ctx->mx_call says so (f5hip_sample)
 int op_of(int precision) { return precision == F5HIP_PREC_FP32 ? OP_F32 : precision == F5HIP_PREC_FP16 ? OP_F16 : OP_F16X3; }
 
+// the checkpoint's rotary frequencies, scaled as `cfg` says, on the device (f5hip_set_long_form, and again after a weight change).  Synchronous.
+int build_long_frequencies(f5hip_ctx* ctx, const f5hip_long_form& cfg) {
+  constexpr int dh = 64, half = dh / 2;  // (f5hip_create takes no other dim_head)
+  float f32[half];
+  double f[half];
+  HIPCHK(hipMemcpy(f32, ctx->inv_freq.p, sizeof(f32), hipMemcpyDeviceToHost));
+  std::copy(f32, f32 + half, f);
+  double amplitude = 1;
+  if (const char* why = scale_rotary_frequencies(f, dh, cfg.rope_scaling, cfg.rope_factor, cfg.rope_original_length, 0, 0, &amplitude))
+    FAIL(F5HIP_ERR_INVALID, "%s", why);
+  HIPCHK(ctx->long_freq.ensure(sizeof(f)));
+  HIPCHK(hipMemcpy(ctx->long_freq.p, f, sizeof(f), hipMemcpyHostToDevice));
+  ctx->long_amplitude = (float)amplitude;
+  return F5HIP_OK;
+}
+
 // ---- finalize: derived layouts -------------------------------------------------------------------
 int finalize_impl(f5hip_ctx* ctx) {
   const auto& c = ctx->cfg;
@@ -734,6 +751,7 @@ int finalize_impl(f5hip_ctx* ctx) {
   HIPCHK(init_convpos_kernels());
   HIPCHK(init_attention_kernels());
   HIPCHK(hipDeviceSynchronize());
+  if (ctx->long_on) CHK(build_long_frequencies(ctx, ctx->long_cfg));
   ctx->finalized = true;
   return F5HIP_OK;
 }
@@ -803,6 +821,24 @@ int prepare_time(f5hip_ctx* ctx, const float* te, const float* coef, int steps, 
   return F5HIP_OK;
 }
 
+// ---- long utterances (f5hip_set_long_form): attention through the operators of operators.h ------------------------------------------
+// q | k | v of one projection are the columns of [rows, 3 H dh]: the operators take them where they are.  S sequences from s0.
+f5hip_window_attention_args long_attention_args(const f5hip_ctx* ctx, int S, int s0, int n, int op, const int32_t* kvlen, void* out) {
+  const auto& c = ctx->cfg;
+  const int64_t inner = (int64_t)c.heads * c.dim_head, eb = op == OP_F16 ? 2 : 4;
+  f5hip_window_attention_args a{};
+  a.dtype = op == OP_F16 ? F5HIP_T_FP16 : F5HIP_T_FP32;
+  a.batch = S; a.q_tokens = a.kv_tokens = n; a.heads = a.kv_heads = c.heads; a.head_dim = c.dim_head;
+  a.window_left = ctx->long_cfg.window_left; a.window_right = ctx->long_cfg.window_right; a.sinks = ctx->long_cfg.sinks;
+  a.scale = 1.0f / sqrtf((float)c.dim_head);
+  char* qkv = ctx->long_qkv.as<char>() + (int64_t)s0 * n * 3 * inner * eb;
+  a.q = qkv; a.k = qkv + inner * eb; a.v = qkv + 2 * inner * eb; a.out = out;
+  for (int64_t* st : {a.q_stride, a.k_stride, a.v_stride}) { st[0] = 3 * inner * n; st[1] = 3 * inner; st[2] = c.dim_head; }
+  a.out_stride[0] = inner * n; a.out_stride[1] = inner; a.out_stride[2] = c.dim_head;
+  a.kv_len = kvlen;
+  return a;
+}
+
 // ---- workspace -----------------------------------------------------------------------------------
 int ensure_workspace(f5hip_ctx* ctx, int B, int n, int nt, int op, bool exact_attn) {
   const auto& c = ctx->cfg;
@@ -848,6 +884,14 @@ int ensure_workspace(f5hip_ctx* ctx, int B, int n, int nt, int op, bool exact_at
       HIPCHK(hipMemset(ctx->vt32.p, 0, ctx->vt32.cap));  // padding columns must be zero for the new row stride
     }
     ENS(scores, (int64_t)2 * B * c.heads * ns * np * 4);
+  } else if (ctx->long_on) {
+    ENS(long_qkv, M * 3 * inner * (op == OP_F16 ? 2 : 4));
+    if (op == OP_F16X3) ENS(long_o, M * inner * 4);
+    if (const char* why = check_window_attention(long_attention_args(ctx, 2 * B, 0, n, op, nullptr, ctx->long_qkv.p))) FAIL(F5HIP_ERR_INVALID, "%s", why);
+    // one chain over all sequences, or two over half of them each (enqueue_steps): the larger of the two
+    const f5hip_window_attention_args all = long_attention_args(ctx, 2 * B, 0, n, op, nullptr, nullptr), half = long_attention_args(ctx, B, 0, n, op, nullptr, nullptr);
+    ctx->long_work_chain = (window_attention_workspace(half) + 255) & ~int64_t(255);
+    ENS(long_work, std::max(std::max(window_attention_workspace(all), 2 * ctx->long_work_chain), int64_t(256)));
   } else {
     const int64_t ldv = (ns + 7) & ~7;
     ENS(q16, M * inner * 2); ENS(k16, M * inner * 2);
@@ -861,7 +905,7 @@ int ensure_workspace(f5hip_ctx* ctx, int B, int n, int nt, int op, bool exact_at
 #undef ENS
   if (moved) ctx->ws_epoch++;
   ctx->ws_B = B;
-  ctx->ws_n = n;
+  ctx->ws_n = ctx->long_on ? 0 : n;  // (the V^T slabs were not prepared for this length)
   ctx->ws_nt = nt;
   return F5HIP_OK;
 }
@@ -1032,6 +1076,44 @@ int run_qkv(f5hip_ctx* ctx, const BlockW& bw, const void* A, int64_t ldA, int M,
     Prof pr(ctx, st, KC_ELEMWISE, 0, 2.0 * M * inner * (4.0 + (exact_attn ? 4.0 : 2.0 * (e.q16_lo ? 2 : 1))));
     HIPCHK(launch_qk_norm_rope(e.q32, e.k32, bw.qn, bw.kn, e.rope_cs, (int64_t)(M / ns) * H * ns, ns, H, dh, c.pe_attn_head, e.qscale, 1e-6f,
                                e.q16, e.q16_lo, e.k16, e.k16_lo, st));
+  }
+  return F5HIP_OK;
+}
+
+// One block's self-attention over S sequences of n frames from s0 (M rows A in the mode's operand layout): the fused q|k|v projection as plain rows,
+// rotary positions of q and k in place, the window, and the out-projection's operand rows in o32 / o_hi.
+int run_long_attention(f5hip_ctx* ctx, const BlockW& bw, const void* A, int64_t ldA, int S, int s0, int n, int op, const int32_t* kvlen, float* o32, f16* o_hi, int br,
+                       int wbytes, hipStream_t st) {
+  const auto& c = ctx->cfg;
+  const int D = c.dim, H = c.heads, dh = c.dim_head, inner = H * dh, M = S * n;
+  float* o = op == OP_F16X3 ? ctx->long_o.as<float>() + (int64_t)s0 * n * inner : o32;
+  f5hip_window_attention_args w = long_attention_args(ctx, S, s0, n, op, kvlen, op == OP_F16 ? (void*)o_hi : (void*)o);
+  w.workspace = ctx->long_work.as<char>() + (br > 0 ? ctx->long_work_chain : 0);
+  w.workspace_bytes = (int64_t)ctx->long_work.cap;
+  {
+    Prof pr(ctx, st, KC_GEMM_BLOCK, gemm_flops(M, 3 * inner, D), (double)M * D * wbytes + 3.0 * inner * D * wbytes + (double)M * 3 * inner * wbytes);
+    GemmCore g = core(A, ldA, wsel(ctx, op, bw.wqkv, bw.wqkv_hi, bw.wqkv_pk), ldA, M, 3 * inner, D);
+    EpiStore e = epi_store(op == OP_F16 ? nullptr : const_cast<float*>(static_cast<const float*>(w.q)), 3 * inner, bw.bqkv);
+    if (op == OP_F16) { e.out16 = const_cast<f16*>(static_cast<const f16*>(w.q)); e.ldo16 = 3 * inner; }
+    HIPCHK(launch_gemm_store(op, g, e, 1, st));
+  }
+  {
+    f5hip_rotary_args r{};
+    r.dtype = w.dtype; r.layout = F5HIP_ROTARY_INTERLEAVED; r.rot_dim = dh;
+    r.batch = S; r.tokens = n; r.heads_q = r.heads_k = H; r.head_dim = dh; r.rot_heads = c.pe_attn_head;
+    r.amplitude = ctx->long_amplitude;
+    r.q = w.q; r.k = w.k; r.q_out = const_cast<void*>(w.q); r.k_out = const_cast<void*>(w.k);
+    for (int i = 0; i < 3; ++i) r.q_stride[i] = r.k_stride[i] = r.q_out_stride[i] = r.k_out_stride[i] = w.q_stride[i];
+    r.inv_freq = ctx->long_freq.as<double>();
+    Prof pr(ctx, st, KC_ELEMWISE, 0, 4.0 * M * inner * (op == OP_F16 ? 2 : 4));
+    HIPCHK(launch_rotary(r, st));
+  }
+  {
+    const double seen = ctx->long_cfg.window_left < 0 || ctx->long_cfg.window_right < 0
+                            ? (double)n : std::min<double>(n, (double)ctx->long_cfg.window_left + ctx->long_cfg.window_right + 1 + ctx->long_cfg.sinks);
+    Prof pr(ctx, st, KC_ATTN, 4.0 * (double)M * inner * seen, 0);
+    HIPCHK(launch_window_attention(w, st));
+    if (op == OP_F16X3) HIPCHK(launch_split_f16_packed(o, M, inner, o_hi, st));
   }
   return F5HIP_OK;
 }
@@ -1214,9 +1296,13 @@ int run_step(f5hip_ctx* ctx, int B, int n, const Stage& sg, int op, bool exact_a
       Prof pr(ctx, st, KC_LNMOD, 0, ln_bytes);
       HIPCHK(launch_layernorm(x, D, M, D, 1e-6f, nullptr, nullptr, md + D, md, a32, a_hi, a_lo, D, st, pkb, ldAb));
     }
-    int qks = QK_PLAIN;
-    CHK(run_qkv(ctx, bw, A, ldAb, M, n, s0, opb, exact_attn, &qks, wbytes, st));
-    CHK(run_attention(ctx, S, s0, n, op, exact_attn, qks, kvlen, o32, o_hi, o_lo, pkb, ldOb, st));
+    if (ctx->long_on) {
+      CHK(run_long_attention(ctx, bw, A, ldAb, S, s0, n, op, kvlen, o32, o_hi, br, wbytes, st));
+    } else {
+      int qks = QK_PLAIN;
+      CHK(run_qkv(ctx, bw, A, ldAb, M, n, s0, opb, exact_attn, &qks, wbytes, st));
+      CHK(run_attention(ctx, S, s0, n, op, exact_attn, qks, kvlen, o32, o_hi, o_lo, pkb, ldOb, st));
+    }
     {  // to_out + mask + gated residual: x += gate_msa * masked(attn) (modules.py:548-556,751)
       Prof pr(ctx, st, KC_GEMM_BLOCK, gemm_flops(M, D, inner), (double)M * inner * wbytes + (double)inner * D * wbytes + 2.0 * M * D * 4);
       GemmCore g = (core(op == OP_F32 ? (const void*)o32 : (const void*)o_hi, ldOb, wsel(ctx, opb, bw.wo, bw.wo_hi, bw.wo_pk, bw.wo_mx), ldOb, M, D, inner));
@@ -1733,7 +1819,7 @@ int f5hip_destroy(f5hip_ctx* ctx) {
                     &ctx->ta, &ctx->th, &ctx->tg, &ctx->sumsq, &ctx->step_cond, &ctx->cconst, &ctx->y, &ctx->h, &ctx->c1, &ctx->x, &ctx->a32,
                     &ctx->a_hi, &ctx->o32, &ctx->o_hi, &ctx->f32, &ctx->f_hi, &ctx->q32, &ctx->k32,
                     &ctx->vt32, &ctx->scores, &ctx->q16, &ctx->k16, &ctx->vt16, &ctx->q16_lo, &ctx->k16_lo, &ctx->vt16_lo, &ctx->vel, &ctx->rope, &ctx->dbg_vel, &ctx->vcol, &ctx->vx,
-                    &ctx->va, &ctx->vh, &ctx->vlogits, &ctx->attn_part, &ctx->attn_stats_buf};
+                    &ctx->va, &ctx->vh, &ctx->vlogits, &ctx->attn_part, &ctx->attn_stats_buf, &ctx->long_freq, &ctx->long_qkv, &ctx->long_o, &ctx->long_work};
   for (DevBuf* b : bufs) b->release();
   ctx->stage.release();
   if (ctx->ev_last) (void)hipEventDestroy(ctx->ev_last);
@@ -1848,6 +1934,28 @@ int f5hip_set_option(f5hip_ctx* ctx, const char* key, int64_t value) {
   return F5HIP_OK;
 }
 
+int f5hip_set_long_form(f5hip_ctx* ctx, const f5hip_long_form* cfg) {
+  if (!ctx) return F5HIP_ERR_INVALID;
+  std::lock_guard<std::mutex> lk(ctx->mu);
+  if (!cfg) {
+    if (ctx->long_on) ctx->ws_epoch++;  // invalidates a captured graph
+    ctx->long_on = false;
+    return F5HIP_OK;
+  }
+  if (ctx->cfg.backbone != 0 || ctx->cfg.qk_norm) FAIL(F5HIP_ERR_UNSUPPORTED, "long form: only the DiT backbone without qk_norm is built");
+  if (!ctx->finalized) FAIL(F5HIP_ERR_STATE, "weights not finalised");
+  constexpr int lim = 1 << 30;
+  if (cfg->window_left < -1 || cfg->window_right < -1 || cfg->sinks < 0 || cfg->window_left >= lim || cfg->window_right >= lim || cfg->sinks >= lim)
+    FAIL(F5HIP_ERR_INVALID, "long form: window_left, window_right >= -1, sinks >= 0, all below 2^30");
+  HIPCHK(hipSetDevice(ctx->device));
+  HIPCHK(hipDeviceSynchronize());  // queued samples read the frequencies that are replaced
+  CHK(build_long_frequencies(ctx, *cfg));
+  ctx->long_cfg = *cfg;
+  ctx->long_on = true;
+  ctx->ws_epoch++;
+  return F5HIP_OK;
+}
+
 int f5hip_attention_stats(f5hip_ctx* ctx, double* out4, int reset) {
   if (!ctx || !out4) return F5HIP_ERR_INVALID;
   std::lock_guard<std::mutex> lk(ctx->mu);
@@ -1926,15 +2034,15 @@ int f5hip_sample(f5hip_ctx* ctx, int B, int n, const float* cond, const uint8_t*
   // MX-corrected scores, qk_scheme_wanted above), 1 force materialised, 2 flash with every operand split, 3 flash with plain fp16 operands
   // in every mode (the default of rounds 2-4), 4 flash with split q, k and plain P, V, 5 = 0 for the half-precision modes, 6 / 7 = 0 with V / V
   // and P as hi + lo halves (round 6: the margin against sharper attention than any golden's)
-  const bool exact_attn = ctx->attn_impl == 1 || (ctx->attn_impl == 0 && (precision == F5HIP_PREC_FP32 || !flash_attn_available()));
-  if (!exact_attn && precision == F5HIP_PREC_FP32) FAIL(F5HIP_ERR_INVALID, "flash attention needs an fp16 precision mode");
+  const bool exact_attn = !ctx->long_on && (ctx->attn_impl == 1 || (ctx->attn_impl == 0 && (precision == F5HIP_PREC_FP32 || !flash_attn_available())));
+  if (!exact_attn && !ctx->long_on && precision == F5HIP_PREC_FP32) FAIL(F5HIP_ERR_INVALID, "flash attention needs an fp16 precision mode");
   const int mel = c.mel_dim, D = c.dim;
   const int64_t BN = (int64_t)B * n;
   // fp16m: MX lines for the block GEMMs where they are built (finalize: mx_ok) and the call is one the pipelined kernel and the flash
   // epilogue take; anything else runs the call in fp16x3 — never less accurate, so the mode needs no error path
   // (the fused q|k|v launch of the pipelined kernel needs >= 8 tokens per sequence; tuning knobs that force a tile without an MX
   // instantiation or the general q|k|v index path take the launches away from it: gemm_mx_tiles_usable)
-  ctx->mx_call = precision == F5HIP_PREC_FP16M && ctx->mx_ok && !exact_attn && ctx->attn_kv_split <= 1 && n >= 8 && gemm_mx_tiles_usable() &&
+  ctx->mx_call = precision == F5HIP_PREC_FP16M && ctx->mx_ok && !exact_attn && !ctx->long_on && ctx->attn_kv_split <= 1 && n >= 8 && gemm_mx_tiles_usable() &&
                  (2 * (BN + B) + 512) * 4 * std::max<int64_t>(std::max<int64_t>(D, c.ff_inner), (int64_t)c.heads * c.dim_head) < (int64_t)0x7ff00000;
 
   // cfg_strength < 1e-5: the reference evaluates only the conditional branch (cfm.py:166-177); otherwise cond + uncond rows are packed
@@ -1988,7 +2096,7 @@ int f5hip_sample(f5hip_ctx* ctx, int B, int n, const float* cond, const uint8_t*
      // (attn_mask_enabled; with it off the reference lets the padding attend, modules.py:511-520) — and only for what is built (DiT, flash)
     int64_t valid = 0;
     for (int b = 0; b < B; ++b) valid += duration[b];
-    const bool packed = ctx->packed_opt && use_mask && c.attn_mask_enabled && c.backbone == 0 && !exact_attn && !c.long_skip_connection && !c.qk_norm &&
+    const bool packed = ctx->packed_opt && use_mask && c.attn_mask_enabled && c.backbone == 0 && !exact_attn && !ctx->long_on && !c.long_skip_connection && !c.qk_norm &&
                         ctx->attn_kv_split <= 1 && valid < BN && n < 65536 && 2 * B < 65536;
     ctx->pk_rows = packed ? nb * valid : 0;
     if (packed) {

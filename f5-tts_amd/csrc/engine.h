@@ -277,6 +277,13 @@ struct f5hip_ctx {
   DevBuf attn_part;
   int attn_stats = 0;          // option "attn_stats": the materialised-score attention accumulates the rows' largest probabilities in
   DevBuf attn_stats_buf;       // attn_stats_buf (4 doubles, f5hip_attention_stats)
+  // f5hip_set_long_form: the blocks' attention through the rotary and sliding-window operators
+  bool long_on = false;
+  f5hip_long_form long_cfg{};
+  float long_amplitude = 1.f;
+  DevBuf long_freq;                    // [dh/2] doubles: the checkpoint's rotary frequencies, scaled
+  DevBuf long_qkv, long_o, long_work;  // q | k | v rows [2B n, 3 H dh] (fp32; fp16 in FP16), fp32 attention rows (FP16X3), partial results
+  int64_t long_work_chain = 0;         // bytes of long_work that one of two concurrent chains uses
   // host inputs of queued copies (the entry points never wait for the stream) and the ordering of calls that arrive on different streams:
   // the workspace is one per context, so a call on a new stream first waits (on the GPU, not the host) for the previous call's work
   HostStage stage;

@@ -106,32 +106,37 @@ const char* check_window_attention(const f5hip_window_attention_args& a) {
   return nullptr;
 }
 
+const char* scale_rotary_frequencies(double* f, int rot_dim, int scaling, double factor, int64_t original_length, double low, double high, double* amplitude) {
+  if (scaling < F5HIP_ROPE_NONE || scaling > F5HIP_ROPE_YARN) return "rotary frequencies: unknown scaling";
+  if (scaling != F5HIP_ROPE_NONE && (!(factor > 0) || !std::isfinite(factor))) return "rotary frequencies: factor must be positive";
+  if (scaling == F5HIP_ROPE_NTK && rot_dim < 4) return "rotary frequencies: the base change needs rot_dim >= 4";
+  if (scaling == F5HIP_ROPE_YARN) {
+    if (low == 0 && high == 0) { low = 1; high = 32; }
+    if (original_length <= 0 || !(low >= 0) || !(high > low) || !std::isfinite(high) || !(factor >= 1))
+      return "rotary frequencies: by parts needs original_length > 0, 0 <= low < high, factor >= 1";
+  }
+  for (int i = 0; i < rot_dim / 2; ++i) {
+    if (scaling == F5HIP_ROPE_LINEAR) f[i] /= factor;
+    if (scaling == F5HIP_ROPE_NTK) f[i] *= std::pow(factor, -2.0 * i / (rot_dim - 2));  // (base factor^(R / (R - 2)))^(-2i / R)
+    if (scaling == F5HIP_ROPE_YARN) {
+      const double r = (double)original_length * f[i] / 6.283185307179586476925;
+      const double g = std::fmin(1.0, std::fmax(0.0, (r - low) / (high - low)));
+      f[i] *= g + (1.0 - g) / factor;
+    }
+  }
+  *amplitude = scaling == F5HIP_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+  return nullptr;
+}
+
 extern "C" {
 int f5hip_rotary_frequencies(int rot_dim, double base, int scaling, double factor, int64_t original_length, double low, double high, double* inv_freq,
                              double* amplitude) {
   if (!inv_freq || !amplitude) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: null pointer");
   if (rot_dim < 2 || (rot_dim & 1)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: rot_dim must be even and >= 2");
   if (!(base > 0) || !std::isfinite(base)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: base must be positive");
-  if (scaling < F5HIP_ROPE_NONE || scaling > F5HIP_ROPE_YARN) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: unknown scaling");
-  if (scaling != F5HIP_ROPE_NONE && (!(factor > 0) || !std::isfinite(factor))) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: factor must be positive");
-  if (scaling == F5HIP_ROPE_NTK && rot_dim < 4) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: the base change needs rot_dim >= 4");
-  if (scaling == F5HIP_ROPE_YARN) {
-    if (low == 0 && high == 0) { low = 1; high = 32; }
-    if (original_length <= 0 || !(low >= 0) || !(high > low) || !std::isfinite(high) || !(factor >= 1))
-      return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary frequencies: by parts needs original_length > 0, 0 <= low < high, factor >= 1");
-  }
-  const double b = scaling == F5HIP_ROPE_NTK ? base * std::pow(factor, (double)rot_dim / (rot_dim - 2)) : base;
-  for (int i = 0; i < rot_dim / 2; ++i) {
-    double f = std::pow(b, -2.0 * i / rot_dim);
-    if (scaling == F5HIP_ROPE_LINEAR) f /= factor;
-    if (scaling == F5HIP_ROPE_YARN) {
-      const double r = (double)original_length * f / 6.283185307179586476925;
-      const double g = std::fmin(1.0, std::fmax(0.0, (r - low) / (high - low)));
-      f *= g + (1.0 - g) / factor;
-    }
-    inv_freq[i] = f;
-  }
-  *amplitude = scaling == F5HIP_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+  for (int i = 0; i < rot_dim / 2; ++i) inv_freq[i] = std::pow(base, -2.0 * i / rot_dim);
+  if (const char* why = scale_rotary_frequencies(inv_freq, rot_dim, scaling, factor, original_length, low, high, amplitude))
+    return f5hip_set_thread_error(F5HIP_ERR_INVALID, why);
   return F5HIP_OK;
 }
 

@@ -171,6 +171,22 @@ class F5HipEngine:
     def set_option(self, key: str, value: int):
         self._chk(self.lib.f5hip_set_option(self._ctx, key.encode(), int(value)))
 
+    def set_long_form(self, window=None, sinks: int = 0, *, rope_scaling: Optional[str] = None, rope_factor: float = 1.0, rope_original_length: int = 0):
+        """Sample long utterances through a sliding window (include/f5hip.h f5hip_set_long_form; DiT backbone): every frame attends to ``window``
+        frames on both sides — an int, or ``(left, right)``; -1: no bound — and to the first ``sinks`` frames (the prompt's), with rotary frequencies
+        scaled for utterances ``rope_factor`` times as long as the ``rope_original_length`` frames the model was trained on (``f5_tts_amd.ops.
+        rotary_frequencies``).  ``set_long_form()`` switches back to attention over the whole utterance."""
+        if window is None and rope_scaling is None:
+            self._chk(self.lib.f5hip_set_long_form(self._ctx, None))
+            return
+        if rope_scaling not in binding.ROPE_SCALINGS:
+            raise ValueError(f"rope_scaling {rope_scaling!r}: one of None, 'linear', 'ntk', 'yarn' is expected")
+        left, right = (-1, -1) if window is None else (window, window) if isinstance(window, int) else window
+        cfg = binding.LongFormC(window_left=left, window_right=right, sinks=sinks, rope_scaling=binding.ROPE_SCALINGS[rope_scaling],
+                                rope_factor=rope_factor, rope_original_length=rope_original_length)
+        with torch.cuda.device(self.device):
+            self._chk(self.lib.f5hip_set_long_form(self._ctx, C.byref(cfg)))
+
     def kernel_stats(self) -> Dict[str, dict]:
         out = {}
         name, calls = C.c_char_p(), C.c_int64()

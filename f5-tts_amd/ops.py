@@ -15,12 +15,11 @@ from typing import Optional, Tuple
 
 import torch
 
-from .binding import F5HipError, check, load_library
+from .binding import ROPE_SCALINGS, F5HipError, check, load_library
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # F5HIP_T_*
 _LAYOUTS = {"interleaved": 0, "half": 1}                          # F5HIP_ROTARY_*
 _ALIGN = {"start": 0, "end": 1}
-_SCALINGS = {None: 0, "none": 0, "linear": 1, "ntk": 2, "yarn": 3}  # F5HIP_ROPE_*
 _ROTARY = struct.Struct("@10if4P12qPP2q")   # f5hip_rotary_args
 _WINDOW = struct.Struct("@11if4P12q3Pq")    # f5hip_window_attention_args
 
@@ -74,11 +73,11 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional
     """``(inv_freq, amplitude)`` for :func:`rotary`: ``rot_dim / 2`` frequencies in 64 bits (on ``device``), scaled for contexts ``factor``
     times as long as trained — ``"linear"`` (positions interpolated), ``"ntk"`` (the base changed) or ``"yarn"`` (by parts: frequencies that turn
     less than ``low`` (1) times over ``original_length`` positions are divided, those above ``high`` (32) kept, mixed between them)."""
-    if scaling not in _SCALINGS:
+    if scaling not in ROPE_SCALINGS:
         raise ValueError(f"scaling {scaling!r}: one of None, 'linear', 'ntk', 'yarn' is expected")
     out, amplitude = (C.c_double * max(1, rot_dim // 2))(), C.c_double()
     lib = load_library()
-    check(lib, None, lib.f5hip_rotary_frequencies(rot_dim, base, _SCALINGS[scaling], factor, original_length, low, high, out, C.byref(amplitude)))
+    check(lib, None, lib.f5hip_rotary_frequencies(rot_dim, base, ROPE_SCALINGS[scaling], factor, original_length, low, high, out, C.byref(amplitude)))
     return torch.tensor(list(out), dtype=torch.float64, device=device), amplitude.value
 
 

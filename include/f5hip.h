@@ -348,6 +348,20 @@ typedef struct f5hip_window_attention_args {
 int64_t f5hip_window_attention_workspace(const f5hip_window_attention_args* args);
 int f5hip_window_attention(const f5hip_window_attention_args* args, int device, void* stream);
 
+/* Long utterances (the DiT backbone without qk_norm): from the next f5hip_sample on, the blocks' self-attention goes through the two operators above — each
+ * frame attends to window_left frames before and window_right behind itself (-1: no bound) and to the first `sinks` frames (the prompt: pass its
+ * frame count), positions rotate by frequencies scaled with rope_scaling (F5HIP_ROPE_*, factor, original length in frames: the longest the model was
+ * trained on).  Attention then costs the window, not the square of the frames.  No counterpart in the reference, whose attention is always over the
+ * whole utterance (model/modules.py:511-520): with windows that hold every frame and no scaling the result is the ordinary one up to rounding.
+ * precision: FP32, and FP16X3 / FP16M (whose block GEMMs then run as FP16X3), attend in fp32; FP16 in fp16.  Options "attn_impl", "attn_kv_split",
+ * "attn_stats" and "packed_rows" have no effect meanwhile.  NULL: off (the default).  After f5hip_finalize_weights; synchronises the device. */
+typedef struct f5hip_long_form {
+  int32_t window_left, window_right, sinks, rope_scaling;
+  double rope_factor;
+  int64_t rope_original_length;
+} f5hip_long_form;
+int f5hip_set_long_form(f5hip_ctx* ctx, const f5hip_long_form* cfg);
+
 /* (The kernel microbenchmarks and fault reproducers — f5hip_bench_* — are not part of the product: include/f5hip_bench.h,
  * libf5hip_bench.so.) */
 
