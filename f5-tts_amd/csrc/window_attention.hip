@@ -41,7 +41,7 @@ hipError_t launch(const WindowArgs& w, const Plan& p, hipStream_t s) {
     constexpr int dp = decltype(DP)::value;
     if (p.few) hipLaunchKernelGGL((window_few_kernel<T, dp>), dim3((unsigned)w.nwg), dim3(64 * FEW_WAVES<T>), 0, s, w);
     else if (p.ranges == 1) hipLaunchKernelGGL((window_rows_kernel<T, dp, 1>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
-    else hipLaunchKernelGGL((window_rows_kernel<T, dp, 2>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
+    else if constexpr (dp == 64) hipLaunchKernelGGL((window_rows_kernel<T, dp, 2>), dim3((unsigned)w.nwg), dim3(256), 0, s, w);
   };
   if (w.dim <= 64) go(std::integral_constant<int, 64>{});
   else if (w.dim <= 96) go(std::integral_constant<int, 96>{});

@@ -8,8 +8,10 @@
 // descriptor's bounds check as zeros).  Only tiles on a border of some row's window take the mask.
 // Product.  S^T = K Q^T on 32x32 matrix instructions leaves a lane 16 keys of ONE query row, so maxima and sums are register work and one
 // half-wave exchange; those registers are, as they stand, the other operand of O^T += V^T P^T (the contraction runs over keys in the
-// accumulator's own order), so P never moves.  V^T fragments come from row-major V tiles by the transposing LDS read (16-bit types) or as
-// single floats.
+// accumulator's own order), so P never moves.  V^T fragments come from row-major V tiles by the transposing LDS read.
+// fp32.  A number is the exact sum of three bf16 pieces of 8 bits each, high | middle | low; a product takes six of the nine piece products (the other
+// three are below 2^-21 of it, below 2^-23 in the mean) on the bf16 matrix instructions, at 6 / 16 of the cost of the fp32 ones.  q is split once, K and V as
+// they are staged, P in registers.
 // Softmax.  exp2(c s - c m) with c = scale log2 e > 0 (a negative scale's sign is folded into q).  m is a reference, not the running maximum, and no
 // maximum is taken on the common path: the weights of a tile are summed anyway, and only where a lane's sum passes 2^15 — the reference is some 2^8 too
 // low, or none has been set — is the tile's maximum taken, O and l rescaled, and the tile's weights computed again.  The reference is set so that the
@@ -72,15 +74,34 @@ struct Win<bf16> {
   }
 };
 template <>
-struct Win<float> {
-  static constexpr float BIAS = 0.0f;
-  static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
-    Frag x, y;
-    x.u = a;
-    y.u = b;
-    Mma32<float>::mma(c, x, y);
+struct Win<float> : Win<bf16> {};  // of the pieces
+
+// two fp32 numbers -> their pieces, a pair a plane.  Truncation: each remainder is exact, and what is left behind the second has 8 bits.
+__device__ __forceinline__ void split_pair(uint32_t x, uint32_t y, uint32_t (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+#ifdef F5_HIPEMU
+    p[i] = (x >> 16) | (y & 0xffff0000u);
+#else
+    p[i] = __builtin_amdgcn_perm(y, x, 0x07060302);  // the high halves
+#endif
+    if (i == 2) break;
+    x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, x) - __builtin_bit_cast(float, x & 0xffff0000u));
+    y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, y) - __builtin_bit_cast(float, y & 0xffff0000u));
   }
-};
+}
+// c += a b over 16 contracted elements of one (16-bit types) or three (fp32) planes, the small products first
+template <typename T>
+__device__ __forceinline__ void mma_planes(f32x16& c, const uint4* a, const uint4* b) {
+  if constexpr (sizeof(T) == 4) {
+    Win<T>::mma(c, a[2], b[0]);
+    Win<T>::mma(c, a[0], b[2]);
+    Win<T>::mma(c, a[1], b[1]);
+    Win<T>::mma(c, a[1], b[0]);
+    Win<T>::mma(c, a[0], b[1]);
+  }
+  Win<T>::mma(c, a[0], b[0]);
+}
 
 // 4 rows of a row-major 16-bit tile, transposed: lanes 4 r + c of a group of 16 name 4 columns (8 bytes) of row r, lane i gets column i of the
 // four rows (ds_read_b64_tr_b16)
@@ -121,14 +142,14 @@ __device__ __forceinline__ BufRsrc tile_rsrc(const char* base, int64_t stride_by
 // the running softmax of one 32-row group: O^T (32 columns a block), reference maximum, row sum
 template <typename T, int DP>
 struct Rows {
-  static constexpr int EB = sizeof(T), ND = DP / 32, NKS = DP * EB / 32;
-  static constexpr int K_ROWB = DP * EB + 16;                              // 32 rows read 16 bytes each without conflicts
-  static constexpr int V_ROWB = EB == 4 ? DP * 4 + 32 : (DP == 64 ? 192 : 320);  // 16 bit: 4 rows start 64 bytes apart in the 256-byte bank row
+  static constexpr int EB = sizeof(T), PL = EB == 4 ? 3 : 1, ND = DP / 32, NKS = DP / 16;  // planes, blocks of 32 columns, steps of 16
+  static constexpr int K_ROWB = DP * 2 + 16;            // of a plane in LDS: 32 rows read 16 bytes each without conflicts
+  static constexpr int V_ROWB = DP == 64 ? 192 : 320;   // 4 rows start 64 bytes apart in the 256-byte bank row
   static constexpr float UNSET = -1e30f, LIMIT = 32768.0f;
   f32x16 o[ND];
   float mc, l;  // c m - BIAS (UNSET: no key seen, any score passes the limit), this lane's share of the row sum
   int lo, hi;      // the lane's row: its window
-  uint4 fq[NKS];
+  uint4 fq[NKS][PL];
 
   __device__ __forceinline__ void reset() {
 #pragma unroll
@@ -137,6 +158,48 @@ struct Rows {
       for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     mc = UNSET;
     l = 0.f;
+  }
+
+  // the lane's row of q: columns 16 k + 8 half .. + 7 for each step, in planes; `negate` flips signs
+  __device__ __forceinline__ void load_q(const T* q, bool live, int dim, int half, uint32_t negate) {
+#pragma unroll
+    for (int k = 0; k < NKS; ++k) {
+      const int col = k * 16 + half * 8;
+      uint4 u[EB / 2];
+#pragma unroll
+      for (int i = 0; i < EB / 2; ++i) {
+        const int at = col + i * (16 / EB);
+        u[i] = live && at < dim ? *reinterpret_cast<const uint4*>(q + at) : make_uint4(0, 0, 0, 0);
+        u[i].x ^= negate; u[i].y ^= negate; u[i].z ^= negate; u[i].w ^= negate;
+      }
+      planes(u, fq[k]);
+    }
+  }
+  // 8 columns as loaded -> operand pieces
+  static __device__ __forceinline__ void planes(const uint4 (&u)[EB / 2], uint4 (&f)[PL]) {
+    if constexpr (EB == 2) {
+      f[0] = u[0];
+    } else {
+      uint32_t p[4][3];
+      split_pair(u[0].x, u[0].y, p[0]);
+      split_pair(u[0].z, u[0].w, p[1]);
+      split_pair(u[1].x, u[1].y, p[2]);
+      split_pair(u[1].z, u[1].w, p[3]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) f[i] = make_uint4(p[0][i], p[1][i], p[2][i], p[3][i]);
+    }
+  }
+  // a 16-byte piece of a K or V row, as loaded -> its place in the planes (plane bytes apart) of row `at`
+  static __device__ __forceinline__ void stage(char* at, int plane, int piece, const uint4& u) {
+    if constexpr (EB == 2) {
+      *reinterpret_cast<uint4*>(at + piece * 16) = u;
+    } else {
+      uint32_t a[3], b[3];
+      split_pair(u.x, u.y, a);
+      split_pair(u.z, u.w, b);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2*>(at + i * plane + piece * 8) = make_uint2(a[i], b[i]);
+    }
   }
 
   // the keys of NB blocks of 32 that the lane's row does not see -> -inf.  `high`, `low`, `sink` (wave-uniform): which borders the tile can
@@ -178,34 +241,25 @@ struct Rows {
     mc = to;
   }
 
-  // A tile is worked through in phases, PHASES_PER_BLOCK for each 32 keys: 16 keys a phase in 16-bit types (the lane's are 16 g + 4 half + 0..3
-  // and 8 on), 8 in fp32 (four registers).  V^T operands of a phase, from V rows at sv:
-  static constexpr int PHASES_PER_BLOCK = EB == 2 ? 2 : 4;
+  // A tile is worked through in phases of 16 keys, two for each 32: the lane's are 16 g + 4 half + 0..3 and 8 on.  V^T operands of a phase, from V rows at
+  // sv (planes `plane` bytes apart):
   struct VFrag {
-    uint4 v[ND];  // 16-bit types: 8 keys of a column; fp32: one key of a column for each of the phase's four registers
+    uint4 v[ND][PL];
   };
-  __device__ __forceinline__ void read_v(VFrag& f, int g, const char* sv, int lane) const {
-    const int half = lane >> 5;
-    if constexpr (EB == 2) {
-      const char* at = sv + (4 * half + ((lane & 15) >> 2)) * V_ROWB + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2 + g * 16 * V_ROWB;
+  static __device__ __forceinline__ void read_v(VFrag& f, int g, const char* sv, int plane, int lane) {
+    const char* at = sv + (g * 16 + 4 * (lane >> 5) + ((lane & 15) >> 2)) * V_ROWB + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const uint2 v0 = lds_read_transposed(at + d * 64), v1 = lds_read_transposed(at + 8 * V_ROWB + d * 64);
-        f.v[d] = make_uint4(v0.x, v0.y, v1.x, v1.y);
-      }
-    } else {
-      const char* at = sv + (4 * half + 8 * g) * V_ROWB + (lane & 31) * 4;
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(at + d * 128);
-        f.v[d] = make_uint4(w[0], w[V_ROWB / 4], w[2 * V_ROWB / 4], w[3 * V_ROWB / 4]);
+      for (int i = 0; i < PL; ++i) {
+        const uint2 v0 = lds_read_transposed(at + i * plane + d * 64), v1 = lds_read_transposed(at + i * plane + 8 * V_ROWB + d * 64);
+        f.v[d][i] = make_uint4(v0.x, v0.y, v1.x, v1.y);
       }
-    }
   }
-  // the weights of a tile's keys, as the second product takes them, and the row sum; the reference raised where it has to be
+  // the weights of a tile's keys, as the second product takes them (pairs, in planes), and the row sum; the reference raised where it has to be
   template <int NB>
   struct Weights {
-    uint32_t p[NB * (EB == 2 ? 8 : 16)];  // 16-bit types: pairs; fp32: one each, in the scores' order
+    uint32_t p[PL][NB * 8];
   };
   template <int NB>
   __device__ __forceinline__ float weights_once(const f32x16 (&s)[NB], Weights<NB>& w, float c) const {
@@ -217,11 +271,13 @@ struct Rows {
         const float x = __builtin_amdgcn_exp2f(fmaf(s[n][r], c, -mc)), y = __builtin_amdgcn_exp2f(fmaf(s[n][r + 1], c, -mc));
         if constexpr (EB == 2) {
           const uint32_t p = Win<T>::pack(x, y);
-          w.p[n * 8 + r / 2] = p;
+          w.p[0][n * 8 + r / 2] = p;
           sum = Win<T>::add2(p, sum);  // of the rounded weights: numerator and denominator see the same ones
         } else {
-          w.p[n * 16 + r] = __builtin_bit_cast(uint32_t, x);
-          w.p[n * 16 + r + 1] = __builtin_bit_cast(uint32_t, y);
+          uint32_t p[3];
+          split_pair(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), p);
+#pragma unroll
+          for (int i = 0; i < PL; ++i) w.p[i][n * 8 + r / 2] = p[i];
           sum += x + y;
         }
       }
@@ -239,18 +295,11 @@ struct Rows {
   // O^T += V^T P^T over phase g's keys
   template <int NB>
   __device__ __forceinline__ void product(const Weights<NB>& w, int g, const VFrag& f) {
-    const uint4 p = make_uint4(w.p[4 * g], w.p[4 * g + 1], w.p[4 * g + 2], w.p[4 * g + 3]);
+    uint4 p[PL];
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      if constexpr (EB == 2) {
-        Win<T>::mma(o[d], f.v[d], p);
-      } else {
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, f.v[d].x), __builtin_bit_cast(float, p.x), o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, f.v[d].y), __builtin_bit_cast(float, p.y), o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, f.v[d].z), __builtin_bit_cast(float, p.z), o[d], 0, 0, 0);
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, f.v[d].w), __builtin_bit_cast(float, p.w), o[d], 0, 0, 0);
-      }
-    }
+    for (int i = 0; i < PL; ++i) p[i] = make_uint4(w.p[i][4 * g], w.p[i][4 * g + 1], w.p[i][4 * g + 2], w.p[i][4 * g + 3]);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) mma_planes<T>(o[d], f.v[d], p);
   }
   __device__ __forceinline__ float reference() const { return mc == UNSET ? -INFINITY : mc; }
 };
@@ -293,8 +342,9 @@ struct Tiles {
 template <typename T, int DP, int KG>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window_rows_kernel(WindowArgs a) {
   using R = Rows<T, DP>;
+  // (fp32 planes are three times as large: 32 keys, or one stage)
   constexpr int KT = sizeof(T) == 2 || KG == 2 ? 64 : 32, NB = KT / 32 / KG, EB = R::EB, CPR = DP * EB / 16, NP = KT * CPR, NL = (NP + 255) / 256, ROWS = 128 / KG;
-  constexpr int KB = KT * R::K_ROWB, VB = KT * R::V_ROWB, STAGES = sizeof(T) == 4 && DP > 64 && KG == 2 ? 1 : 2;
+  constexpr int KPL = KT * R::K_ROWB, VPL = KT * R::V_ROWB, KB = R::PL * KPL, VB = R::PL * VPL, STAGES = sizeof(T) == 4 && KG == 2 ? 1 : 2;
   __shared__ __attribute__((aligned(16))) char smem[STAGES * (KB + VB)];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, ql = lane & 31;
   int L = xcd_order((int)blockIdx.x, a.nwg);
@@ -322,14 +372,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
   st.reset();
   st.lo = sp.low(p0 + tok);
   st.hi = live ? sp.high(p0 + tok) : 0;
-  const T* qp = static_cast<const T*>(a.q) + b * a.q_stride[0] + tok * a.q_stride[1] + head * a.q_stride[2];
-#pragma unroll
-  for (int k = 0; k < R::NKS; ++k) {
-    const int col = (k * 32 + half * 16) / EB;
-    uint4 u = live && col < a.dim ? *reinterpret_cast<const uint4*>(qp + col) : make_uint4(0, 0, 0, 0);
-    u.x ^= a.negate; u.y ^= a.negate; u.z ^= a.negate; u.w ^= a.negate;
-    st.fq[k] = u;
-  }
+  st.load_q(static_cast<const T*>(a.q) + b * a.q_stride[0] + tok * a.q_stride[1] + head * a.q_stride[2], live, a.dim, half, a.negate);
 
   const int64_t ksb = a.k_stride[1] * EB, vsb = a.v_stride[1] * EB;
   const int dimb = a.dim * EB;
@@ -357,8 +400,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
     for (int i = 0; i < NL; ++i) {
       const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
       if (NP % 256 == 0 || c < NP) {
-        *reinterpret_cast<uint4*>(smem + slot * (KB + VB) + r * R::K_ROWB + col * 16) = rk[i];
-        *reinterpret_cast<uint4*>(smem + slot * (KB + VB) + KB + r * R::V_ROWB + col * 16) = rv[i];
+        R::stage(smem + slot * (KB + VB) + r * R::K_ROWB, KPL, col, rk[i]);
+        R::stage(smem + slot * (KB + VB) + KB + r * R::V_ROWB, VPL, col, rv[i]);
       }
     }
   };
@@ -373,25 +416,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
-    // Operands are read from LDS one step ahead of the matrix instructions that take them — four (three) K pieces, or the V pieces of a phase — and the scheduling
+    // Operands are read from LDS one step ahead of the matrix instructions that take them — one to four steps of K, or the V pieces of a phase — and the scheduling
     // barriers keep the compiler from sinking the reads back to their uses (a wave then sits out an LDS round trip at each).
-    constexpr int QS = NB * R::NKS % 4 == 0 ? 4 : 3, NQ = NB * R::NKS / QS, PH = NB * R::PHASES_PER_BLOCK;
+    constexpr int QS = R::PL == 3 ? 1 : NB * R::NKS % 4 == 0 ? 4 : 3, NQ = NB * R::NKS / QS, PH = 2 * NB;
     static_assert(NB * R::NKS % QS == 0, "whole steps of K pieces");
-    uint4 fk[2][QS];
+    uint4 fk[2][QS][R::PL];
     const auto read_k = [&](auto C) {
       constexpr int q = decltype(C)::value;
 #pragma unroll
-      for (int i = 0; i < QS; ++i) fk[q & 1][i] = *reinterpret_cast<const uint4*>(sk + (QS * q + i) / R::NKS * 32 * R::K_ROWB + (QS * q + i) % R::NKS * 32);
+      for (int i = 0; i < QS; ++i)
+#pragma unroll
+        for (int p = 0; p < R::PL; ++p)
+          fk[q & 1][i][p] = *reinterpret_cast<const uint4*>(sk + p * KPL + (QS * q + i) / R::NKS * 32 * R::K_ROWB + (QS * q + i) % R::NKS * 32);
     };
     typename R::VFrag fv[2];
     read_k(std::integral_constant<int, 0>{});
     static_for<NQ>([&](auto Q) {
       constexpr int q = decltype(Q)::value;
       if constexpr (q + 1 < NQ) read_k(std::integral_constant<int, q + 1>{});
-      else st.read_v(fv[0], 0, sv, lane);
+      else R::read_v(fv[0], 0, sv, VPL, lane);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < QS; ++i) Win<T>::mma(s[(QS * q + i) / R::NKS], fk[q & 1][i], st.fq[(QS * q + i) % R::NKS]);
+      for (int i = 0; i < QS; ++i) mma_planes<T>(s[(QS * q + i) / R::NKS], fk[q & 1][i], st.fq[(QS * q + i) % R::NKS]);
       __builtin_amdgcn_sched_barrier(0);
     });
     st.mask(s, key0, t.kend, half, key0 + 32 * NB > min(whi0, t.kend), key0 < wlo1 && key0 + 32 * NB > a.sinks, a.sinks);
@@ -399,7 +445,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
     st.weigh(s, w, c);
     static_for<PH>([&](auto G) {
       constexpr int g = decltype(G)::value;
-      if constexpr (g + 1 < PH) st.read_v(fv[(g + 1) & 1], g + 1, sv, lane);
+      if constexpr (g + 1 < PH) R::read_v(fv[(g + 1) & 1], g + 1, sv, VPL, lane);
       __builtin_amdgcn_sched_barrier(0);
       st.product(w, g, fv[g & 1]);
       __builtin_amdgcn_sched_barrier(0);
@@ -484,7 +530,7 @@ template <typename T, int DP>
 __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(WindowArgs a) {
   using R = Rows<T, DP>;
   constexpr int NW = FEW_WAVES<T>, KT = 32, EB = R::EB, CPR = DP * EB / 16, NL = KT * CPR / 64;
-  constexpr int VB = KT * R::V_ROWB, MERGE = NW * 32 * 33 * 4;
+  constexpr int VPL = KT * R::V_ROWB, VB = R::PL * VPL, MERGE = NW * 32 * 33 * 4, EK = EB / 2;  // EK: 16-byte loads of a lane's 8 columns of K
   __shared__ __attribute__((aligned(16))) char smem[NW * VB > MERGE ? NW * VB : MERGE];
   __shared__ float sml[NW][32][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, ql = lane & 31;
@@ -509,14 +555,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
   st.reset();
   st.lo = sp.low(p0 + tok);
   st.hi = live ? sp.high(p0 + tok) : 0;
-  const T* qp = static_cast<const T*>(a.q) + b * a.q_stride[0] + tok * a.q_stride[1] + head * a.q_stride[2];
-#pragma unroll
-  for (int k = 0; k < R::NKS; ++k) {
-    const int col = (k * 32 + half * 16) / EB;
-    uint4 u = live && col < a.dim ? *reinterpret_cast<const uint4*>(qp + col) : make_uint4(0, 0, 0, 0);
-    u.x ^= a.negate; u.y ^= a.negate; u.z ^= a.negate; u.w ^= a.negate;
-    st.fq[k] = u;
-  }
+  st.load_q(static_cast<const T*>(a.q) + b * a.q_stride[0] + tok * a.q_stride[1] + head * a.q_stride[2], live, a.dim, half, a.negate);
   const char* kb = static_cast<const char*>(a.k) + (b * a.k_stride[0] + kvh * a.k_stride[2]) * EB;
   const char* vb = static_cast<const char*>(a.v) + (b * a.v_stride[0] + kvh * a.v_stride[2]) * EB;
   const int64_t ksb = a.k_stride[1] * EB, vsb = a.v_stride[1] * EB;
@@ -527,10 +566,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
     key0 = t < na ? t * KT : bb + (t - na) * KT;
     kend = t < na ? ea : khigh;
   };
-  uint4 fk[R::NKS], rv[NL];
-  uint32_t ok[R::NKS], ov[NL];
+  uint4 fk[R::NKS][EK], rv[NL];
+  uint32_t ok[R::NKS][EK], ov[NL];
 #pragma unroll
-  for (int k = 0; k < R::NKS; ++k) ok[k] = k * 32 + half * 16 < dimb ? (uint32_t)(ql * (int)ksb + k * 32 + half * 16) : OOB_ROW;
+  for (int k = 0; k < R::NKS; ++k)
+#pragma unroll
+    for (int i = 0; i < EK; ++i) {
+      const int col = (k * 16 + half * 8) * EB + i * 16;  // bytes
+      ok[k][i] = col < dimb ? (uint32_t)(ql * (int)ksb + col) : OOB_ROW;
+    }
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
     const int c = lane + i * 64, r = c / CPR, col = c - r * CPR;
@@ -541,7 +585,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
     tile(t, key0, kend);
     const BufRsrc Kr = tile_rsrc(kb, ksb, key0, min(KT, kend - key0), dimb);
 #pragma unroll
-    for (int k = 0; k < R::NKS; ++k) fk[k] = buffer_load_b128(Kr, ok[k]);
+    for (int k = 0; k < R::NKS; ++k)
+#pragma unroll
+      for (int i = 0; i < EK; ++i) fk[k][i] = buffer_load_b128(Kr, ok[k][i]);
   };
   const auto load_v = [&](int t) {
     int key0, kend;
@@ -561,13 +607,17 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
 #pragma unroll
-    for (int k = 0; k < R::NKS; ++k) Win<T>::mma(s[0], fk[k], st.fq[k]);
+    for (int k = 0; k < R::NKS; ++k) {
+      uint4 f[R::PL];
+      R::planes(fk[k], f);
+      mma_planes<T>(s[0], f, st.fq[k]);
+    }
     if (t + NW < t1) load_k(t + NW);  // as soon as its registers are free
     wave_lds_sync();                  // the last tile's reads of these rows come before
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int c = lane + i * 64, r = c / CPR, col = c - r * CPR;
-      *reinterpret_cast<uint4*>(sv + r * R::V_ROWB + col * 16) = rv[i];
+      R::stage(sv + r * R::V_ROWB, VPL, col, rv[i]);
     }
     if (t + NW < t1) load_v(t + NW);
     st.mask(s, key0, kend, half, key0 + KT > min(high0, kend), key0 < low1 && key0 + KT > a.sinks, a.sinks);
@@ -575,9 +625,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
     st.weigh(s, w, a.scale_log2);
     wave_lds_sync();
 #pragma unroll
-    for (int g = 0; g < R::PHASES_PER_BLOCK; ++g) {
+    for (int g = 0; g < 2; ++g) {
       typename R::VFrag f;
-      st.read_v(f, g, sv, lane);
+      R::read_v(f, g, sv, VPL, lane);
       st.product(w, g, f);
     }
   }
