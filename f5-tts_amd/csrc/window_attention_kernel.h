@@ -234,9 +234,7 @@ struct Rows {
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     const float to = fmaxf(mc, fmaf(both_halves_max(mx), c, -Win<T>::BIAS)), al = __builtin_amdgcn_exp2f(mc - to);
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] *= al;
+    for (int d = 0; d < ND; ++d) o[d] *= al;
     l *= al;
     mc = to;
   }
@@ -327,16 +325,9 @@ __device__ __forceinline__ int spread_units(int i, int n) {
 // ---- many rows: K and V tiles of 64 keys shared through LDS, two stages ------------------------------------------------------------------------------
 // Four waves: 4 / KG groups of 32 rows x KG ranges of keys.  KG = 1: 128 rows a workgroup, a wave takes whole tiles.  KG = 2: 64 rows, a wave takes one half
 // of every tile and the two halves' results meet in LDS at the end — twice the workgroups, each half as long, where row blocks alone load the CUs unevenly.
-// The tiles of a row block in order: keys [0, ea), then [bb, high).  One cursor walks them for the loads, one for the work; advancing costs a few scalar
-// instructions where indexing by a tile number took ninety.
+// The tiles of a row block in order: keys [0, ea), then [bb, khigh).
 struct Tiles {
   int key0, kend;  // the tile's first key, its range's end
-  int bb, high;
-  template <int KT>
-  __device__ __forceinline__ void next() {
-    key0 += KT;
-    if (key0 >= kend && kend != high) { key0 = bb; kend = high; }
-  }
 };
 
 template <typename T, int DP, int KG>
@@ -387,9 +378,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
   }
   const char* kb = static_cast<const char*>(a.k) + (b * a.k_stride[0] + kvh * a.k_stride[2]) * EB;
   const char* vb = static_cast<const char*>(a.v) + (b * a.v_stride[0] + kvh * a.v_stride[2]) * EB;
-  const auto load = [&](const Tiles& t) {
-    const int rows = min(KT, t.kend - t.key0);
-    const BufRsrc Kr = tile_rsrc(kb, ksb, t.key0, rows, dimb), Vr = tile_rsrc(vb, vsb, t.key0, rows, dimb);
+  Tiles ahead{t0 < na ? t0 * KT : bb + (t0 - na) * KT, t0 < na ? ea : khigh};  // the tile to load next, and where its rows are
+  const char *kp = kb + ahead.key0 * ksb, *vp = vb + ahead.key0 * vsb;
+  const int64_t kstep = KT * ksb, vstep = KT * vsb;
+  const auto advance = [&] {
+    ahead.key0 += KT;
+    kp += kstep;
+    vp += vstep;
+    if (ahead.key0 >= ahead.kend && ahead.kend != khigh) {
+      ahead = Tiles{bb, khigh};
+      kp = kb + bb * ksb;
+      vp = vb + bb * vsb;
+    }
+  };
+  const auto load = [&] {
+    const int rows = min(KT, ahead.kend - ahead.key0);
+    const BufRsrc Kr = make_rsrc(kp, (uint32_t)((rows - 1) * (int)ksb + dimb)), Vr = make_rsrc(vp, (uint32_t)((rows - 1) * (int)vsb + dimb));
 #pragma unroll
     for (int i = 0; i < NL; ++i) rk[i] = buffer_load_b128(Kr, ok[i]);
 #pragma unroll
@@ -452,22 +456,31 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
     });
   };
   if (t0 < t1) {
-    Tiles at{t0 < na ? t0 * KT : bb + (t0 - na) * KT, t0 < na ? ea : khigh, bb, khigh}, ahead = at;
-    load(at);
+    Tiles at = ahead;
+    load();
     store(0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
       const int slot = STAGES == 2 ? (t - t0) & 1 : 0;
-      ahead.next<KT>();
-      if (t + 1 < t1) load(ahead);
+      const bool more = t + 1 < t1;
+      if (more) {
+        advance();
+        load();
+      }
       work(at, slot);
       if constexpr (STAGES == 1) __syncthreads();  // every wave has read the one stage
-      if (t + 1 < t1) store(STAGES == 2 ? slot ^ 1 : 0);
+      if (more) store(STAGES == 2 ? slot ^ 1 : 0);
       __syncthreads();
       at = ahead;
     }
   }
 
+#ifndef F5_HIPEMU
+  // O as one register tuple behind the loop: left to itself the compiler gathers what the epilogue reads inside the loop, 32 moves behind every tile's
+  // matrix instructions
+#pragma unroll
+  for (int d = 0; d < R::ND; ++d) asm volatile("" : "+v"(st.o[d]));
+#endif
   float l = both_halves_sum(st.l), top = st.reference();
   if constexpr (KG == 2) {  // the second half's result through LDS (its places have been read: the loop ended at a barrier), columns as the lanes hold them
     constexpr int LANE_FLOATS = 16 * R::ND + 2;
