@@ -145,7 +145,7 @@ struct Rows {
   static constexpr int EB = sizeof(T), PL = EB == 4 ? 3 : 1, ND = DP / 32, NKS = DP / 16;  // planes, blocks of 32 columns, steps of 16
   static constexpr int K_ROWB = DP * 2 + 16;            // of a plane in LDS: 32 rows read 16 bytes each without conflicts
   static constexpr int V_ROWB = DP == 64 ? 192 : 320;   // 4 rows start 64 bytes apart in the 256-byte bank row
-  static constexpr float UNSET = -1e30f, LIMIT = 32768.0f;
+  static constexpr float UNSET = -3.402823466e38f, LIMIT = 32768.0f;
   f32x16 o[ND];
   float mc, l;  // c m - BIAS (UNSET: no key seen, any score passes the limit), this lane's share of the row sum
   int lo, hi;      // the lane's row: its window

@@ -328,6 +328,9 @@ int f5hip_rotary(const f5hip_rotary_args* args, int device, void* stream);
  * (negative: no bound; window_right = 0: causal; the sinks are exempt from the left bound only).  out = softmax(scale q . k) v over the
  * keys seen; a query that sees none gives zeros.  Query head h reads key head h / (heads / kv_heads).  Scores, softmax statistics and sums
  * are fp32; with 16-bit types the weights are rounded to that type for the product with v (the softmax sum is that of the rounded weights).
+ * Scores have to stay below 2^22 in magnitude (an fp32 dot product of that size has lost the differences a softmax reads).
+ * fp32 tensors are multiplied as three bf16 pieces a number, six products of nine: fp32 accuracy for finite numbers; an infinity that is seen gives
+ * NaN.  `out` shares no memory with q, k and v.
  *   kv_len, q_len   device int32 [batch] or NULL (kv_tokens / q_tokens), clamped into [0, kv_tokens] / [0, q_tokens].  Output rows
  *                   i >= q_len[b] are left as they were.  Keys at and past kv_len[b] and keys in front of every query's window are not
  *                   read, whatever they hold; a v row that SOME query of the call sees has to be finite for the others' sake.

@@ -182,3 +182,19 @@ def check_attention(ops, to, case, seed=0, spread=1.0, scale=None):
     assert over(out, ref, tol) <= 1
     assert (out.cpu()[~rows] == 0).all()
     return out
+
+
+def check_huge_scores(ops, to):
+    """Scores down to -2 million, each row one-hot by a margin of 32 768: the first key of a row's window.  16-bit types: the weight cancels against
+    the sum up to 2^-22 of a 16-bit number, so exactly; fp32: six of nine piece products (2^-21), the division and two products (2^-23 each)."""
+    for dtype in ("bf16", "fp16", "fp32"):
+        for n, m in ((70, 70), (70, 2)):
+            q = torch.full((1, m, 2, 64), 2.0 ** 6).to(TYPES[dtype])
+            k = (-(torch.arange(n) + 1.0) * 2.0 ** 6)[None, :, None, None].expand(1, n, 2, 64).contiguous().to(TYPES[dtype])
+            v = torch.randn(1, n, 2, 64, generator=torch.Generator().manual_seed(1)).to(TYPES[dtype])
+            out = ops.window_attention(to(q), to(k), to(v), window=(20, 0), align="end").cpu()
+            first = (torch.arange(m) + n - m - 20).clamp_min(0)
+            if dtype == "fp32":
+                assert torch.allclose(out[0], v[0, first], rtol=2.0 ** -20, atol=0)
+            else:
+                assert torch.equal(out[0], v[0, first])

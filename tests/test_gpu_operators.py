@@ -94,6 +94,10 @@ def test_window_attention_sharp_scores(name):
     O.check_attention(ops, gpu, O.ATTENTION[name], seed=3, scale=-1.0)
 
 
+def test_window_attention_of_huge_scores():
+    O.check_huge_scores(ops, gpu)
+
+
 def test_window_attention_ignores_what_nobody_sees():
     check_unseen(ops, gpu)
 

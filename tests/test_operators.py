@@ -175,6 +175,11 @@ def test_window_attention_ignores_what_nobody_sees_on_the_shim(host):
     check_unseen(host, same)
 
 
+@shim
+def test_window_attention_of_huge_scores_on_the_shim(host):
+    O.check_huge_scores(host, same)
+
+
 def check_unseen(ops_, to):
     """Keys and values behind the last key, and in front of every window but no sink, may hold NaN and infinities."""
     for name in ("token_grouped", "chunk", "token_fp32", "ragged"):
