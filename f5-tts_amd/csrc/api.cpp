@@ -887,7 +887,6 @@ int ensure_workspace(f5hip_ctx* ctx, int B, int n, int nt, int op, bool exact_at
   } else if (ctx->long_on) {
     ENS(long_qkv, M * 3 * inner * (op == OP_F16 ? 2 : 4));
     if (op == OP_F16X3) ENS(long_o, M * inner * 4);
-    if (const char* why = check_window_attention(long_attention_args(ctx, 2 * B, 0, n, op, nullptr, ctx->long_qkv.p))) FAIL(F5HIP_ERR_INVALID, "%s", why);
     // one chain over all sequences, or two over half of them each (enqueue_steps): the larger of the two
     const f5hip_window_attention_args all = long_attention_args(ctx, 2 * B, 0, n, op, nullptr, nullptr), half = long_attention_args(ctx, B, 0, n, op, nullptr, nullptr);
     ctx->long_work_chain = (window_attention_workspace(half) + 255) & ~int64_t(255);
@@ -2021,6 +2020,8 @@ int f5hip_sample(f5hip_ctx* ctx, int B, int n, const float* cond, const uint8_t*
   if (!cond || !cond_mask || !text || !duration || !y0 || !t || !out) FAIL(F5HIP_ERR_INVALID, "null argument");
   if (B <= 0 || n <= 0 || steps <= 0 || nt <= 0) FAIL(F5HIP_ERR_INVALID, "batch, n, nt and steps must be positive");
   if (n > 8192 && ctx->cfg.conv_layers > 0) FAIL(F5HIP_ERR_INVALID, "n=%d exceeds the 8192-frame text position table (dit.py:47)", n);
+  if (ctx->long_on && (2 * (int64_t)B * ctx->cfg.heads >= (1 << 22) || 2 * (int64_t)B * ctx->cfg.heads * n >= (1 << 30)))
+    FAIL(F5HIP_ERR_INVALID, "long form: 2 x batch x heads must be below 2^22, times the frames below 2^30");  // f5hip_window_attention's limits
   if (ode_method != 0 && ode_method != 1) FAIL(F5HIP_ERR_UNSUPPORTED, "ode_method %d: only euler (0) and midpoint (1) are built", ode_method);
   if (precision < F5HIP_PREC_FP32 || precision > F5HIP_PREC_FP16M) FAIL(F5HIP_ERR_INVALID, "bad precision %d", precision);
   for (int b = 0; b < B; ++b)

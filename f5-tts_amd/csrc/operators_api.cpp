@@ -20,6 +20,12 @@ bool strides_ok(const int64_t (&st)[3], const int64_t (&ext)[3], bool output) {
   }
   return true;
 }
+// an output that starts where its input does has the input's strides
+bool in_place_or_apart(const void* in, const void* out, const int64_t (&si)[3], const int64_t (&so)[3], const int64_t (&ext)[3]) {
+  for (int i = 0; i < 3; ++i)
+    if (in == out && ext[i] > 1 && si[i] != so[i]) return false;
+  return true;
+}
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
 // the calling thread's device while an operator launches, restored on every path
@@ -71,6 +77,9 @@ const char* check_rotary(const f5hip_rotary_args& a) {
   if (!strides_ok(a.q_stride, eq, false) || !strides_ok(a.q_out_stride, eq, true) ||
       (a.heads_k && (!strides_ok(a.k_stride, ek, false) || !strides_ok(a.k_out_stride, ek, true))))
     return "rotary: strides must lie in [0, 2^40], an output's must not be 0";
+  if (!in_place_or_apart(a.q, a.q_out, a.q_stride, a.q_out_stride, eq) ||
+      (a.heads_k && (!in_place_or_apart(a.k, a.k_out, a.k_stride, a.k_out_stride, ek) || a.q_out == a.k || a.k_out == a.q || a.q_out == a.k_out)))
+    return "rotary: an output may be its own input with the same strides, or memory of its own";
   if (a.position_stride < 0 || a.position_stride > (int64_t(1) << 40)) return "rotary: position_stride must lie in [0, 2^40]";
   return nullptr;
 }
@@ -92,6 +101,7 @@ const char* check_window_attention(const f5hip_window_attention_args& a) {
   if ((int64_t)a.batch * a.heads * a.q_tokens >= lim) return "window attention: batch * heads * q_tokens must be below 2^30";
   if (a.batch == 0 || a.q_tokens == 0) return nullptr;
   if (!a.q || !a.out || (a.kv_tokens && (!a.k || !a.v))) return "window attention: null pointer";
+  if (a.out == a.q || (a.kv_tokens && (a.out == a.k || a.out == a.v))) return "window attention: out must share no memory with q, k and v";
   if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16)) return "window attention: pointers must be aligned to 16 bytes";
   if (!aligned(a.kv_len, 4) || !aligned(a.q_len, 4)) return "window attention: lengths must be aligned to 4 bytes";
   const int64_t eq[3] = {a.batch, a.q_tokens, a.heads}, ek[3] = {a.batch, a.kv_tokens, a.kv_heads};

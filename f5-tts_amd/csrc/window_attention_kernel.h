@@ -683,7 +683,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
         if (col == 0) { a.part_ml[part * 2] = rtop; a.part_ml[part * 2 + 1] = rl; }
       } else {
         T* op = static_cast<T*>(a.out) + b * a.out_stride[0] + otok * a.out_stride[1] + ohead * a.out_stride[2];
-        op[col] = (T)(rl > 0.f ? x / rl : 0.f);
+        op[col] = (T)(rl > 0.f ? x / rl : x * 0.f);  // nothing seen: 0; a NaN seen: NaN
       }
     }
   }

@@ -176,6 +176,8 @@ class F5HipEngine:
         frames on both sides — an int, or ``(left, right)``; -1: no bound — and to the first ``sinks`` frames (the prompt's), with rotary frequencies
         scaled for utterances ``rope_factor`` times as long as the ``rope_original_length`` frames the model was trained on (``f5_tts_amd.ops.
         rotary_frequencies``).  ``set_long_form()`` switches back to attention over the whole utterance."""
+        if window is None and sinks:
+            raise ValueError("sinks need a window: without one every frame attends to all of them")
         if window is None and rope_scaling is None:
             self._chk(self.lib.f5hip_set_long_form(self._ctx, None))
             return

@@ -138,7 +138,7 @@ def check_graph_and_chains(engines):
 
 def check_refusals(engines):
     eng = engines("tiny", 1)
-    for kw in (dict(window=(-2, 0)), dict(window=4, sinks=-1), dict(window=1 << 30), dict(window=4, rope_scaling="cubic"),
+    for kw in (dict(sinks=5), dict(window=(-2, 0)), dict(window=4, sinks=-1), dict(window=1 << 30), dict(window=4, rope_scaling="cubic"),
                dict(window=4, rope_scaling="linear", rope_factor=0.0), dict(window=4, rope_scaling="yarn", rope_factor=2.0)):
         with pytest.raises(ValueError):
             eng.set_long_form(**kw)

@@ -198,3 +198,15 @@ def check_huge_scores(ops, to):
                 assert torch.allclose(out[0], v[0, first], rtol=2.0 ** -20, atol=0)
             else:
                 assert torch.equal(out[0], v[0, first])
+
+
+def check_seen_nan(ops, to):
+    """A NaN that a row sees is its result, whatever form the sizes take; a row of q reaches no other row."""
+    for name in ("token_fp32", "token_grouped", "three_tokens_odd_group", "chunk", "both_sides", "fp32_both_sides", "both_sides_bf16_128"):
+        q, k, v, kw = attention_inputs(ATTENTION[name])
+        ref, tol, rows = attention(q, k, v, **kw)
+        q[0, -1, 1] = math.nan
+        out = ops.window_attention(to(q), to(k), to(v), **{x: to(y) if isinstance(y, torch.Tensor) else y for x, y in kw.items()}).cpu()
+        assert out[0, -1, 1].isnan().all()
+        out[0, -1, 1] = ref[0, -1, 1].to(out.dtype)
+        assert over(out, ref, tol) <= 1

@@ -98,6 +98,10 @@ def test_window_attention_of_huge_scores():
     O.check_huge_scores(ops, gpu)
 
 
+def test_window_attention_of_a_nan():
+    O.check_seen_nan(ops, gpu)
+
+
 def test_window_attention_ignores_what_nobody_sees():
     check_unseen(ops, gpu)
 

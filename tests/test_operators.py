@@ -110,6 +110,27 @@ def test_window_attention_refuses(host):
             host.window_attention(a.pop("q"), a.pop("k"), a.pop("v"), **a)
 
 
+def test_outputs_that_overlap_are_refused(host):
+    f, x = O.frequencies(64), q4(2, 4, 2, 64)
+    y = q4(2, 4, 2, 64)
+    host.rotary(x, y, f, out=(x, y))
+    for out in ((y, x), (x, x), (y, q4(2, 4, 2, 64)), (q4(2, 4, 2, 64), x), (x.view(2, 2, 4, 64).transpose(1, 2), y)):
+        with pytest.raises(ValueError, match="own input"):
+            host.rotary(x, y, f, out=out)
+    for i in range(3):
+        qkv = [q4(2, 4, 2, 64) for _ in range(3)]
+        with pytest.raises(ValueError, match="no memory"):
+            host.window_attention(*qkv, out=qkv[i])
+
+
+def test_numbers_past_fp32_are_refused(host):
+    x = q4(1, 4, 2, 64)
+    with pytest.raises(ValueError):
+        host.rotary(x, None, O.frequencies(64), amplitude=1e39)
+    with pytest.raises(ValueError):
+        host.window_attention(x, x, x, scale=1e39)
+
+
 def test_c_entries_refuse_null_and_say_why():
     lib = binding.load_library()
     assert lib.f5hip_rotary(None, 0, None) == 1 and b"null" in lib.f5hip_last_error(None)
@@ -178,6 +199,11 @@ def test_window_attention_ignores_what_nobody_sees_on_the_shim(host):
 @shim
 def test_window_attention_of_huge_scores_on_the_shim(host):
     O.check_huge_scores(host, same)
+
+
+@shim
+def test_window_attention_of_a_nan_on_the_shim(host):
+    O.check_seen_nan(host, same)
 
 
 def check_unseen(ops_, to):
