@@ -6,8 +6,8 @@
 namespace {
 // Few rows (window_few_kernel: waves along the keys) up to 32 rows of a key head, many (window_rows_kernel: waves along the rows) above.
 // Many rows: 128 rows a workgroup, or, up to 64 columns and where that makes fewer than four workgroups a CU, 64 rows whose two waves share the keys
-// (KG = 2).  Measured on an MI355X: 2 x 1406 frames, 16 heads of 64, 1026 keys seen (352 blocks of 128 rows) 24 us with 64 rows, 33 us with 128; 16 ragged
-// utterances of 12 heads (1920 blocks) 59 and 48 us; 2 x 8192 frames (2048 blocks) 170 and 148 us; with 128 columns (6 chunks of 200 tokens, 32 heads on 8,
+// (KG = 2).  Measured on an MI355X: 2 x 1406 frames, 16 heads of 64, 1026 keys seen (352 blocks of 128 rows) 23 us with 64 rows, 33 us with 128; 16 ragged
+// utterances of 12 heads (1920 blocks) 56 and 50 us; 2 x 8192 frames (2048 blocks) 157 and 148 us; with 128 columns (6 chunks of 200 tokens, 32 heads on 8,
 // 336 blocks) 81 and 75 us: there the tiles are twice as large, and loading them for 64 rows costs more than the better balance brings.
 // Ranges of keys over workgroups, joined by window_join_kernel, where the blocks alone leave CUs without two workgroups: at least 256 keys each (few
 // rows: 512, two tiles a wave).  More ranges balance better and lose it to the partial results' way out and back (the chunks in two ranges 75 us, three 81,
@@ -71,6 +71,8 @@ hipError_t launch_window_attention(const f5hip_window_attention_args& a, hipStre
   w.negate = a.scale < 0 ? (a.dtype == F5HIP_T_FP32 ? 0x80000000u : 0x80008000u) : 0u;
   w.nblk = p.nblk; w.nsplit = p.nsplit;
   w.nwg = (int)((int64_t)a.batch * a.kv_heads * p.nblk * p.nsplit);
+  const int units = a.batch * a.kv_heads;
+  w.xcd_units = units % 8 == 0 && units <= 64 ? units / 8 : 0;
   w.part_o = static_cast<float*>(a.workspace);
   w.part_ml = w.part_o ? w.part_o + parts(a, p) * a.head_dim : nullptr;
   if (a.dtype == F5HIP_T_FP16) return launch<f16>(w, p, s);

@@ -34,6 +34,7 @@ struct WindowArgs {
   float scale_log2;       // |scale| log2(e), > 0
   uint32_t negate;        // sign bits to flip in q (a negative scale)
   int nblk, nsplit, nwg;  // row blocks of a (sequence, key head), key ranges of a row block, workgroups
+  int xcd_units;          // (sequence, key head) units of each XCD whose blocks take turns; 0: one unit after the other
   float *part_o, *part_ml;  // nsplit > 1: [rows, nsplit, dim] unnormalised, [rows, nsplit, 2] (c m - BIAS, l); rows = (sequence, head, token)
 };
 
@@ -111,6 +112,21 @@ __device__ __forceinline__ uint2 lds_read_transposed(const char* p) {
 #else
   typedef short s16x4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+#endif
+}
+
+// 16 bytes a lane from a buffer to LDS, lane l's at p + 16 l (p wave-uniform); what lies past the descriptor's end arrives as zeros
+__device__ __forceinline__ void load_to_lds(BufRsrc r, uint32_t offset, char* p) {
+#ifdef F5_HIPEMU
+  const uint4 v = buffer_load_b128(r, offset);
+  memcpy(p + 16 * hipemu::blk->cur->lane, &v, 16);
+#else
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)p, 16, (int)offset, 0, 0, 0);
+#endif
+}
+__device__ __forceinline__ void loads_to_lds_landed() {  // the wave's; a barrier makes them the workgroup's
+#ifndef F5_HIPEMU
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #endif
 }
 
@@ -254,6 +270,16 @@ struct Rows {
         f.v[d][i] = make_uint4(v0.x, v0.y, v1.x, v1.y);
       }
   }
+  // ... from rows without padding whose places are exchanged (window_rows_kernel): `at` holds the lane's place of each column block
+  template <int ROWB>
+  static __device__ __forceinline__ void read_v_exchanged(VFrag& f, int g, const char* sv, const uint32_t (&at)[ND]) {
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const char* p = sv + at[d] + g * 16 * ROWB;
+      const uint2 v0 = lds_read_transposed(p), v1 = lds_read_transposed(p + 8 * ROWB);
+      f.v[d][0] = make_uint4(v0.x, v0.y, v1.x, v1.y);
+    }
+  }
   // the weights of a tile's keys, as the second product takes them (pairs, in planes), and the row sum; the reference raised where it has to be
   template <int NB>
   struct Weights {
@@ -322,26 +348,60 @@ __device__ __forceinline__ int spread_units(int i, int n) {
   return i < big ? (i % (q + 1)) * 8 + i / (q + 1) : ((i - big) % q) * 8 + r + (i - big) / q;
 }
 
+// A workgroup's place in the order.  Blocks of rows go from the last one down: later tokens see more keys (a window cut off at the sequence's start is
+// shorter), so what is left for the end of the launch is short.  Where every XCD has up to eight whole units, their blocks take turns, for the same reason (2 x 1406
+// frames of 16 heads, 4 units an XCD: 22.3 -> 20.4 us, in fp32 79 -> 70 us; 2 x 8192 frames 142 -> 138 us); with more, a unit's blocks would be so far apart in
+// time that its keys leave L2 between them (16 utterances of 12 heads, 24 units: 45 us one unit after the other, 49 us in turns).
+struct Place {
+  int ks, blk, bh;
+};
+__device__ __forceinline__ Place place_of(const WindowArgs& a, int block) {
+  Place p;
+  int i;
+  if (a.xcd_units) {
+    const int l = block >> 3;
+    p.ks = l % a.nsplit;
+    i = l / a.nsplit;
+    p.bh = i % a.xcd_units * 8 + (block & 7);
+    i /= a.xcd_units;
+  } else {
+    const int l = xcd_order(block, a.nwg);
+    p.ks = l % a.nsplit;
+    i = l / a.nsplit;
+    p.bh = spread_units(i / a.nblk, a.batch * a.kv_heads);
+    i %= a.nblk;
+  }
+  p.blk = a.nblk - 1 - i;
+  return p;
+}
+
 // ---- many rows: K and V tiles of 64 keys shared through LDS, two stages ------------------------------------------------------------------------------
 // Four waves: 4 / KG groups of 32 rows x KG ranges of keys.  KG = 1: 128 rows a workgroup, a wave takes whole tiles.  KG = 2: 64 rows, a wave takes one half
 // of every tile and the two halves' results meet in LDS at the end — twice the workgroups, each half as long, where row blocks alone load the CUs unevenly.
 // The tiles of a row block in order: keys [0, ea), then [bb, khigh).
+// 16-bit tiles go from memory to LDS without registers on the way (2 x 8192 frames of 16 heads of 64: 148 -> 142 us, and the 40 registers saved make room for
+// a fourth workgroup a CU: 139 us).  Such loads write 64 lanes' pieces side by side, so rows have no padding; instead the pieces of a row change places by its
+// number — K: 16 bytes by all 8 or 16 places, so that 16 rows read at one column hit 16 different places of the 256-byte bank row; V: 64 bytes, so that the 4
+// rows of a transposing read do — in the addresses that are loaded and in those that are read.  Rows of up to 96 and 128 columns take 256 bytes.
 struct Tiles {
   int key0, kend;  // the tile's first key, its range's end
 };
 
 template <typename T, int DP, int KG>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window_rows_kernel(WindowArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 64 ? 4 : sizeof(T) == 4 && DP > 64 ? 1 : 2) void window_rows_kernel(WindowArgs a) {
   using R = Rows<T, DP>;
   // (fp32 planes are three times as large: 32 keys, or one stage)
-  constexpr int KT = sizeof(T) == 2 || KG == 2 ? 64 : 32, NB = KT / 32 / KG, EB = R::EB, CPR = DP * EB / 16, NP = KT * CPR, NL = (NP + 255) / 256, ROWS = 128 / KG;
-  constexpr int KPL = KT * R::K_ROWB, VPL = KT * R::V_ROWB, KB = R::PL * KPL, VB = R::PL * VPL, STAGES = sizeof(T) == 4 && KG == 2 ? 1 : 2;
-  __shared__ __attribute__((aligned(16))) char smem[STAGES * (KB + VB)];
+  constexpr bool DMA = sizeof(T) == 2;
+  constexpr int EB = R::EB, KT = DMA || KG == 2 ? 64 : 32, NB = KT / 32 / KG, ROWS = 128 / KG, STAGES = DMA || KG == 1 ? 2 : 1;
+  constexpr int ROWB = DP == 64 ? 128 : 256, CPR = DMA ? ROWB / 16 : DP * EB / 16, NP = KT * CPR, NL = (NP + 255) / 256;  // pieces of 16 bytes: a row's, a tile's, a thread's
+  constexpr int KPL = KT * (DMA ? ROWB : R::K_ROWB), VPL = KT * (DMA ? ROWB : R::V_ROWB), KB = R::PL * KPL, VB = R::PL * VPL;
+  static_assert(!DMA || NP % 256 == 0, "whole wave instructions");
+  // (an array a stage: the compiler then sees that what is read now is not what is being loaded)
+  __shared__ __attribute__((aligned(1024))) char stage0[KB + VB];
+  __shared__ __attribute__((aligned(1024))) char stage1[STAGES == 2 ? KB + VB : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, ql = lane & 31;
-  int L = xcd_order((int)blockIdx.x, a.nwg);
-  const int ks = L % a.nsplit;
-  L /= a.nsplit;
-  const int blk = L % a.nblk, bh = spread_units(L / a.nblk, a.batch * a.kv_heads), b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
+  const Place pl = place_of(a, (int)blockIdx.x);
+  const int ks = pl.ks, blk = pl.blk, b = pl.bh / a.kv_heads, kvh = pl.bh - b * a.kv_heads;
   const int n = a.kv_len ? max(0, min(a.kv_len[b], a.tk)) : a.tk, nq = a.q_len ? max(0, min(a.q_len[b], a.tq)) : a.tq;
   const int first = blk * ROWS / a.group;
   if (first >= nq) return;  // (the whole workgroup: no barrier has been reached)
@@ -367,14 +427,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
 
   const int64_t ksb = a.k_stride[1] * EB, vsb = a.v_stride[1] * EB;
   const int dimb = a.dim * EB;
-  uint4 rk[NL], rv[NL];
+  uint4 rk[NL], rv[NL];     // (fp32)
   uint32_t ok[NL], ov[NL];  // the thread's pieces of a tile (rows past its last key are past the descriptor's end, columns past the head's are put there)
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
-    const bool in = col * 16 < dimb && (NP % 256 == 0 || c < NP);
-    ok[i] = in ? (uint32_t)(r * (int)ksb + col * 16) : OOB_ROW;
-    ov[i] = in ? (uint32_t)(r * (int)vsb + col * 16) : OOB_ROW;
+    const int c = tid + i * 256, r = c / CPR, at = c - r * CPR;
+    const int ck = DMA ? at ^ (DP == 64 ? r >> 1 & 7 : r & 15) : at, cv = DMA ? at ^ (DP == 64 ? r >> 1 & 1 : r & 3) * 4 : at;
+    const bool in = NP % 256 == 0 || c < NP;
+    ok[i] = in && ck * 16 < dimb ? (uint32_t)(r * (int)ksb + ck * 16) : OOB_ROW;
+    ov[i] = in && cv * 16 < dimb ? (uint32_t)(r * (int)vsb + cv * 16) : OOB_ROW;
+  }
+  uint32_t atk[R::NKS], atv[R::ND];  // (16-bit types) the lane's places of its K pieces and V blocks in a tile
+#pragma unroll
+  for (int k = 0; k < R::NKS; ++k) atk[k] = (kg * 32 * NB + ql) * ROWB + ((2 * k + half) ^ (DP == 64 ? ql >> 1 & 7 : ql & 15)) * 16;
+#pragma unroll
+  for (int d = 0; d < R::ND; ++d) {
+    const int r = (lane & 15) >> 2;
+    atv[d] = (kg * 32 * NB + 4 * half + r) * ROWB + (d ^ (DP == 64 ? r >> 1 : r)) * 64 + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
   }
   const char* kb = static_cast<const char*>(a.k) + (b * a.k_stride[0] + kvh * a.k_stride[2]) * EB;
   const char* vb = static_cast<const char*>(a.v) + (b * a.v_stride[0] + kvh * a.v_stride[2]) * EB;
@@ -391,30 +460,43 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
       vp = vb + bb * vsb;
     }
   };
-  const auto load = [&] {
+  const auto place = [&](auto S) { return decltype(S)::value ? stage1 : stage0; };
+  const auto load = [&](auto S) {  // (a row's last piece may lie past the descriptor's end: zeros)
     const int rows = min(KT, ahead.kend - ahead.key0);
     const BufRsrc Kr = make_rsrc(kp, (uint32_t)((rows - 1) * (int)ksb + dimb)), Vr = make_rsrc(vp, (uint32_t)((rows - 1) * (int)vsb + dimb));
+    if constexpr (DMA) {
+      char* to = place(S) + wave * 1024;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) rk[i] = buffer_load_b128(Kr, ok[i]);
+      for (int i = 0; i < NL; ++i) load_to_lds(Kr, ok[i], to + i * 4096);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) rv[i] = buffer_load_b128(Vr, ov[i]);
+      for (int i = 0; i < NL; ++i) load_to_lds(Vr, ov[i], to + KB + i * 4096);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) rk[i] = buffer_load_b128(Kr, ok[i]);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) rv[i] = buffer_load_b128(Vr, ov[i]);
+    }
   };
-  const auto store = [&](int slot) {
+  const auto store = [&](auto S) {
+    if constexpr (DMA) {
+      loads_to_lds_landed();
+    } else {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
-      if (NP % 256 == 0 || c < NP) {
-        R::stage(smem + slot * (KB + VB) + r * R::K_ROWB, KPL, col, rk[i]);
-        R::stage(smem + slot * (KB + VB) + KB + r * R::V_ROWB, VPL, col, rv[i]);
+      for (int i = 0; i < NL; ++i) {
+        const int c = tid + i * 256, r = c / CPR, col = c - r * CPR;
+        if (NP % 256 == 0 || c < NP) {
+          R::stage(place(S) + r * R::K_ROWB, KPL, col, rk[i]);
+          R::stage(place(S) + KB + r * R::V_ROWB, VPL, col, rv[i]);
+        }
       }
     }
   };
   const float c = a.scale_log2;
-  const auto work = [&](const Tiles& t, int slot) {
+  const auto work = [&](const Tiles& t, auto S) {
     const int key0 = t.key0 + kg * 32 * NB;  // the wave's keys of the tile
     if (key0 >= min(whi1, t.kend) || (min(key0 + 32 * NB, t.kend) <= wlo0 && key0 >= a.sinks)) return;  // none of its rows sees one (wave-uniform)
-    const char* sk = smem + slot * (KB + VB) + (kg * 32 * NB + ql) * R::K_ROWB + half * 16;
-    const char* sv = smem + slot * (KB + VB) + KB + kg * 32 * NB * R::V_ROWB;
+    const char* sk = place(S) + (DMA ? 0 : (kg * 32 * NB + ql) * R::K_ROWB + half * 16);
+    const char* sv = place(S) + KB + (DMA ? 0 : kg * 32 * NB * R::V_ROWB);
     f32x16 s[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -431,14 +513,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
       for (int i = 0; i < QS; ++i)
 #pragma unroll
         for (int p = 0; p < R::PL; ++p)
-          fk[q & 1][i][p] = *reinterpret_cast<const uint4*>(sk + p * KPL + (QS * q + i) / R::NKS * 32 * R::K_ROWB + (QS * q + i) % R::NKS * 32);
+          fk[q & 1][i][p] = *reinterpret_cast<const uint4*>(sk + p * KPL + (QS * q + i) / R::NKS * 32 * (DMA ? ROWB : R::K_ROWB) +
+                                                            (DMA ? atk[(QS * q + i) % R::NKS] : (QS * q + i) % R::NKS * 32));
+    };
+    const auto read_v = [&](typename R::VFrag& f, int g) {
+      if constexpr (DMA) R::template read_v_exchanged<ROWB>(f, g, sv, atv);
+      else R::read_v(f, g, sv, VPL, lane);
     };
     typename R::VFrag fv[2];
     read_k(std::integral_constant<int, 0>{});
     static_for<NQ>([&](auto Q) {
       constexpr int q = decltype(Q)::value;
       if constexpr (q + 1 < NQ) read_k(std::integral_constant<int, q + 1>{});
-      else R::read_v(fv[0], 0, sv, VPL, lane);
+      else read_v(fv[0], 0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < QS; ++i) mma_planes<T>(s[(QS * q + i) / R::NKS], fk[q & 1][i], st.fq[(QS * q + i) % R::NKS]);
@@ -449,7 +536,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
     st.weigh(s, w, c);
     static_for<PH>([&](auto G) {
       constexpr int g = decltype(G)::value;
-      if constexpr (g + 1 < PH) R::read_v(fv[(g + 1) & 1], g + 1, sv, VPL, lane);
+      if constexpr (g + 1 < PH) read_v(fv[(g + 1) & 1], g + 1);
       __builtin_amdgcn_sched_barrier(0);
       st.product(w, g, fv[g & 1]);
       __builtin_amdgcn_sched_barrier(0);
@@ -457,21 +544,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
   };
   if (t0 < t1) {
     Tiles at = ahead;
-    load();
-    store(0);
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-      const int slot = STAGES == 2 ? (t - t0) & 1 : 0;
+    constexpr std::integral_constant<int, 0> S0{};
+    constexpr std::integral_constant<int, STAGES - 1> S1{};
+    const auto step = [&](int t, auto S, auto next) {
       const bool more = t + 1 < t1;
       if (more) {
         advance();
-        load();
+        load(next);
       }
-      work(at, slot);
+      work(at, S);
       if constexpr (STAGES == 1) __syncthreads();  // every wave has read the one stage
-      if (more) store(STAGES == 2 ? slot ^ 1 : 0);
+      if (more) store(next);
       __syncthreads();
       at = ahead;
+    };
+    load(S0);
+    store(S0);
+    __syncthreads();
+    for (int t = t0; t < t1; t += STAGES) {
+      step(t, S0, S1);
+      if (STAGES == 2 && t + 1 < t1) step(t + 1, S1, S0);
     }
   }
 
@@ -484,8 +576,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void window
   float l = both_halves_sum(st.l), top = st.reference();
   if constexpr (KG == 2) {  // the second half's result through LDS (its places have been read: the loop ended at a barrier), columns as the lanes hold them
     constexpr int LANE_FLOATS = 16 * R::ND + 2;
-    static_assert(STAGES * (KB + VB) >= 2 * 64 * LANE_FLOATS * 4, "the halves meet in the tiles' place");
-    float* x = reinterpret_cast<float*>(smem) + wave / 2 * 64 * LANE_FLOATS + lane;
+    static_assert(KB + VB >= (3 - STAGES) * 64 * LANE_FLOATS * 4, "the halves meet in the tiles' place");
+    float* x = reinterpret_cast<float*>(wave >= 2 && STAGES == 2 ? stage1 : stage0) + (STAGES == 1 ? wave / 2 * 64 * LANE_FLOATS : 0) + lane;
     if (kg == 1) {
 #pragma unroll
       for (int d = 0; d < R::ND; ++d)
@@ -547,10 +639,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES<T>, 1) void window_few_kernel(Window
   __shared__ __attribute__((aligned(16))) char smem[NW * VB > MERGE ? NW * VB : MERGE];
   __shared__ float sml[NW][32][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, ql = lane & 31;
-  int L = xcd_order((int)blockIdx.x, a.nwg);
-  const int ks = L % a.nsplit;
-  L /= a.nsplit;
-  const int blk = L % a.nblk, bh = spread_units(L / a.nblk, a.batch * a.kv_heads), b = bh / a.kv_heads, kvh = bh - b * a.kv_heads;
+  const Place pl = place_of(a, (int)blockIdx.x);
+  const int ks = pl.ks, blk = pl.blk, b = pl.bh / a.kv_heads, kvh = pl.bh - b * a.kv_heads;
   const int n = a.kv_len ? max(0, min(a.kv_len[b], a.tk)) : a.tk, nq = a.q_len ? max(0, min(a.q_len[b], a.tq)) : a.tq;
   const int first = blk * 32 / a.group;
   if (first >= nq) return;  // (the whole workgroup)
