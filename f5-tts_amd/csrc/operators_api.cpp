@@ -20,6 +20,28 @@ bool strides_ok(const int64_t (&st)[3], const int64_t (&ext)[3], bool output) {
   }
   return true;
 }
+// an axis of at most one element may carry any stride: none
+void drop_idle_strides(int64_t (&st)[3], int64_t batch, int64_t tokens, int64_t heads) {
+  if (batch <= 1) st[0] = 0;
+  if (tokens <= 1) st[1] = 0;
+  if (heads <= 1) st[2] = 0;
+}
+f5hip_rotary_args plain(const f5hip_rotary_args& args) {
+  f5hip_rotary_args a = args;
+  drop_idle_strides(a.q_stride, a.batch, a.tokens, a.heads_q);
+  drop_idle_strides(a.q_out_stride, a.batch, a.tokens, a.heads_q);
+  drop_idle_strides(a.k_stride, a.batch, a.tokens, a.heads_k);
+  drop_idle_strides(a.k_out_stride, a.batch, a.tokens, a.heads_k);
+  return a;
+}
+f5hip_window_attention_args plain(const f5hip_window_attention_args& args) {
+  f5hip_window_attention_args a = args;
+  drop_idle_strides(a.q_stride, a.batch, a.q_tokens, a.heads);
+  drop_idle_strides(a.out_stride, a.batch, a.q_tokens, a.heads);
+  drop_idle_strides(a.k_stride, a.batch, a.kv_tokens, a.kv_heads);
+  drop_idle_strides(a.v_stride, a.batch, a.kv_tokens, a.kv_heads);
+  return a;
+}
 // an output that starts where its input does has the input's strides
 bool in_place_or_apart(const void* in, const void* out, const int64_t (&si)[3], const int64_t (&so)[3], const int64_t (&ext)[3]) {
   for (int i = 0; i < 3; ++i)
@@ -150,26 +172,28 @@ int f5hip_rotary_frequencies(int rot_dim, double base, int scaling, double facto
   return F5HIP_OK;
 }
 
-int f5hip_rotary(const f5hip_rotary_args* a, int device, void* stream) {
-  if (!a) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary: null argument");
-  if (const char* why = check_rotary(*a)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, why);
-  if (a->batch == 0 || a->tokens == 0) return F5HIP_OK;
-  return on_device(device, [&] { return launch_rotary(*a, (hipStream_t)stream); });
+int f5hip_rotary(const f5hip_rotary_args* args, int device, void* stream) {
+  if (!args) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "rotary: null argument");
+  const f5hip_rotary_args a = plain(*args);
+  if (const char* why = check_rotary(a)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, why);
+  if (a.batch == 0 || a.tokens == 0) return F5HIP_OK;
+  return on_device(device, [&] { return launch_rotary(a, (hipStream_t)stream); });
 }
 
-int64_t f5hip_window_attention_workspace(const f5hip_window_attention_args* a) {
-  const char* why = a ? check_window_attention(*a) : "window attention: null argument";
+int64_t f5hip_window_attention_workspace(const f5hip_window_attention_args* args) {
+  const char* why = args ? check_window_attention(plain(*args)) : "window attention: null argument";
   if (why) { f5hip_set_thread_error(F5HIP_ERR_INVALID, why); return -1; }
-  return a->batch == 0 || a->q_tokens == 0 ? 0 : window_attention_workspace(*a);
+  return args->batch == 0 || args->q_tokens == 0 ? 0 : window_attention_workspace(*args);
 }
 
-int f5hip_window_attention(const f5hip_window_attention_args* a, int device, void* stream) {
-  if (!a) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "window attention: null argument");
-  if (const char* why = check_window_attention(*a)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, why);
-  if (a->batch == 0 || a->q_tokens == 0) return F5HIP_OK;
-  const int64_t need = window_attention_workspace(*a);
-  if (a->workspace_bytes < need || (need && (!a->workspace || !aligned(a->workspace, 16))))
+int f5hip_window_attention(const f5hip_window_attention_args* args, int device, void* stream) {
+  if (!args) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "window attention: null argument");
+  const f5hip_window_attention_args a = plain(*args);
+  if (const char* why = check_window_attention(a)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, why);
+  if (a.batch == 0 || a.q_tokens == 0) return F5HIP_OK;
+  const int64_t need = window_attention_workspace(a);
+  if (a.workspace_bytes < need || (need && (!a.workspace || !aligned(a.workspace, 16))))
     return f5hip_set_thread_error(F5HIP_ERR_INVALID, "window attention: workspace missing, too small or not aligned to 16 bytes");
-  return on_device(device, [&] { return launch_window_attention(*a, (hipStream_t)stream); });
+  return on_device(device, [&] { return launch_window_attention(a, (hipStream_t)stream); });
 }
 }  // extern "C"

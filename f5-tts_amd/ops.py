@@ -33,10 +33,6 @@ def _device(t: torch.Tensor) -> Tuple[int, int]:
     return index, torch._C._cuda_getCurrentRawStream(index)  # torch.cuda.current_stream(device).cuda_stream without the Python objects (2 us)
 
 
-def _strides(shape, stride) -> Tuple[int, int, int]:
-    return (stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0, stride[2] if shape[2] > 1 else 0)  # an axis of one element may carry any stride
-
-
 def _tensor(name: str, t: torch.Tensor, dtype: Optional[torch.dtype] = None, device: Optional[torch.device] = None) -> None:
     if not isinstance(t, torch.Tensor) or t.dim() != 4:
         raise ValueError(f"{name}: a [batch, tokens, heads, head_dim] tensor is expected")
@@ -47,10 +43,6 @@ def _tensor(name: str, t: torch.Tensor, dtype: Optional[torch.dtype] = None, dev
         raise ValueError(f"{name}: {t.dtype} on {t.device}, the first tensor is {dtype} on {device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the operators are for inference (use torch.no_grad())")
-
-
-def _empty(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _lengths(name: str, t: Optional[torch.Tensor], like: torch.Tensor) -> Optional[torch.Tensor]:
@@ -106,13 +98,14 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
         if kshape[0] != b or kshape[1] != n or kshape[3] != d or hk == 0:
             raise ValueError(f"k is {tuple(kshape)}, q {tuple(shape)}: batch, tokens and head_dim must agree")
     if out is None:
-        q = q if q.stride(3) == 1 else q.contiguous()
-        q_out = _empty(q)
-        if k is None:
-            k_out = None
-        else:
-            k = k if k.stride(3) == 1 else k.contiguous()
-            k_out = _empty(k)
+        if q.stride(3) != 1:
+            q = q.contiguous()
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_out = None
+        if k is not None:
+            if k.stride(3) != 1:
+                k = k.contiguous()
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
         q_out, k_out = out
         for name, x, y in (("q", q, q_out), ("k", k, k_out)):
@@ -133,12 +126,11 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
         positions = positions.contiguous()
         step = n if positions.dim() == 2 and positions.shape[0] > 1 else 0
     device, stream = _device(q)
-    qs, qos = _strides(shape, q.stride()), _strides(shape, q_out.stride())
-    ks, kos, kp, kop = ((0, 0, 0), (0, 0, 0), 0, 0) if k is None else \
-        (_strides(kshape, k.stride()), _strides(kshape, k_out.stride()), k.data_ptr(), k_out.data_ptr())
+    zero = (0, 0, 0)
     args = _pack(_ROTARY, (_TYPES[dtype], _LAYOUTS[layout], 1 if inverse else 0, 2 * inv_freq.shape[0], b, n, h, hk, d,
-                           -1 if rot_heads is None else rot_heads, amplitude, q.data_ptr(), kp, q_out.data_ptr(), kop, *qs, *ks, *qos, *kos,
-                           inv_freq.data_ptr(), 0 if positions is None else positions.data_ptr(), step, offset))
+                           -1 if rot_heads is None else rot_heads, amplitude, q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(),
+                           0 if k is None else k_out.data_ptr(), *q.stride()[:3], *(zero if k is None else k.stride()[:3]), *q_out.stride()[:3],
+                           *(zero if k is None else k_out.stride()[:3]), inv_freq.data_ptr(), 0 if positions is None else positions.data_ptr(), step, offset))
     lib = load_library()
     status = lib.f5hip_rotary(args, device, stream)
     if status:
@@ -146,14 +138,16 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
     return q_out, k_out
 
 
-def _rows(t: torch.Tensor, shape) -> Tuple[torch.Tensor, Tuple[int, int, int]]:
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, int, int, int]]:
     """The tensor, or a copy, with 16-byte aligned rows, and its strides."""
-    stride = t.stride()
-    st = _strides(shape, stride)
-    if stride[3] == 1 and ((st[0] | st[1] | st[2]) * t.element_size() | t.data_ptr()) % 16 == 0:
-        return t, st
+    st = t.stride()
+    if st[3] == 1:
+        if ((st[0] | st[1] | st[2]) * t.element_size() | t.data_ptr()) % 16 == 0:
+            return t, st
+        if t.data_ptr() % 16 == 0 and all(m <= 1 or x * t.element_size() % 16 == 0 for x, m in zip(st[:3], t.shape)):
+            return t, st  # an axis of one element may carry any stride
     t = t.clone(memory_format=torch.contiguous_format)
-    return t, _strides(shape, t.stride())
+    return t, t.stride()
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: Tuple[int, int] = (-1, -1), sinks: int = 0,
@@ -182,20 +176,20 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     kv_len, q_len = _lengths("kv_len", kv_len, q), _lengths("q_len", q_len, q)
     left, right = window
     if out is None:
-        out = _empty(q) if q_len is None else torch.zeros(shape, dtype=dtype, device=where)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_len is None else torch.zeros(shape, dtype=dtype, device=where)
     else:
         _tensor("out", out, dtype, where)
         if out.shape != shape:
             raise ValueError(f"out is {tuple(out.shape)}, q {tuple(shape)}")
         if out.stride(3) != 1:
             raise ValueError("out: the last axis must be contiguous")
-    q, qs = _rows(q, shape)
-    k, ks = _rows(k, kshape)
-    v, vs = _rows(v, kshape)
+    q, qs = _rows(q)
+    k, ks = _rows(k)
+    v, vs = _rows(v)
     device, stream = _device(q)
     lib = load_library()
     fields = [_TYPES[dtype], b, n, kshape[1], h, kshape[2], d, left, right, sinks, _ALIGN[align], d ** -0.5 if scale is None else scale,
-              q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *qs, *ks, *vs, *_strides(shape, out.stride()),
+              q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *qs[:3], *ks[:3], *vs[:3], *out.stride()[:3],
               0 if kv_len is None else kv_len.data_ptr(), 0 if q_len is None else q_len.data_ptr(), 0, 0]
     args = _pack(_WINDOW, fields)
     need = lib.f5hip_window_attention_workspace(args)

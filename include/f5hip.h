@@ -286,8 +286,8 @@ int f5hip_reset_kernel_stats(f5hip_ctx* ctx);
  * context: every buffer, the workspace included, is the caller's, nothing is kept from one call for the next, and calls from any number of
  * threads, streams and captured graphs are independent as long as their buffers are.  `device` is the HIP device ordinal the pointers
  * belong to; the calling thread's current device is restored.  Errors: f5hip_last_error(NULL), per thread.
- * Tensors are [batch, tokens, heads, head_dim] with any strides of the first three axes (in elements; 0 = broadcast, inputs only), the
- * last axis contiguous. */
+ * Tensors are [batch, tokens, heads, head_dim] with any strides of the first three axes (in elements; 0 = broadcast, inputs only; of an
+ * axis of one element any), the last axis contiguous. */
 enum { F5HIP_T_FP32 = 0, F5HIP_T_FP16 = 1, F5HIP_T_BF16 = 2 };
 enum { F5HIP_ROTARY_INTERLEAVED = 0 /* pairs (2i, 2i + 1) */, F5HIP_ROTARY_HALF = 1 /* pairs (i, i + rot_dim / 2) */ };
 enum { F5HIP_ROPE_NONE = 0, F5HIP_ROPE_LINEAR = 1, F5HIP_ROPE_NTK = 2, F5HIP_ROPE_YARN = 3 };

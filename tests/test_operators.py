@@ -202,6 +202,19 @@ def test_window_attention_of_huge_scores_on_the_shim(host):
 
 
 @shim
+def test_axes_of_one_element_carry_any_stride_on_the_shim(host):
+    x = torch.randn(128, generator=torch.Generator().manual_seed(4)).half()
+    plain, odd = x.view(1, 1, 2, 64), x.as_strided((1, 1, 2, 64), (7, (1 << 40) + 3, 64, 1))
+    f = O.frequencies(64)
+    assert torch.equal(host.rotary(odd, odd, f, offset=3)[1], host.rotary(plain, None, f, offset=3)[0])
+    assert torch.equal(host.window_attention(odd, odd, odd), host.window_attention(plain, plain, plain))
+    out, one = torch.zeros(64).half().as_strided((1, 1, 1, 64), (0, 0, 3, 1)), plain[:, :, :1]
+    assert torch.equal(host.window_attention(one, one, one, out=out), host.window_attention(one, one, one))
+    fits = x.as_strided((1, 1, 2, 64), (7, 3, 64, 1))
+    assert ops._rows(fits)[0] is fits  # not copied
+
+
+@shim
 def test_window_attention_of_a_nan_on_the_shim(host):
     O.check_seen_nan(host, same)
 
