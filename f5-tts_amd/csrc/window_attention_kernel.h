@@ -502,9 +502,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 64 ? 4 : sizeof(T) == 
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[nb][r] = 0.f;
-    // Operands are read from LDS one step ahead of the matrix instructions that take them — one to four steps of K, or the V pieces of a phase — and the scheduling
+    // Operands are read from LDS one step ahead of the matrix instructions that take them — one or two steps of K, or the V pieces of a phase — and the scheduling
     // barriers keep the compiler from sinking the reads back to their uses (a wave then sits out an LDS round trip at each).
-    constexpr int QS = R::PL == 3 ? 1 : NB * R::NKS % 4 == 0 ? 4 : 3, NQ = NB * R::NKS / QS, PH = 2 * NB;
+    constexpr int QS = R::PL == 3 ? 1 : 2, NQ = NB * R::NKS / QS, PH = 2 * NB;
     static_assert(NB * R::NKS % QS == 0, "whole steps of K pieces");
     uint4 fk[2][QS][R::PL];
     const auto read_k = [&](auto C) {

@@ -87,6 +87,17 @@ def test_window_attention_larger(case):
     O.check_attention(ops, gpu, case, seed=5)
 
 
+@pytest.mark.parametrize("case", [
+    (1, 1, 3000, 16, 16, 64, "fp16", -1, 0, 0, "end", None, None),
+    (2, 40, 2000, 16, 4, 128, "bf16", 1500, 0, 9, "end", [2000, 1203], [40, 33]),
+    (8, 200, 600, 8, 1, 64, "fp16", -1, 0, 0, "end", [600, 200, 0, 599, 1, 64, 65, 333], None),
+    (4, 170, 900, 4, 2, 64, "fp32", 700, 30, 20, "start", [900, 170, 20, 450], None),
+], ids=lambda c: "-".join(map(str, c[:7])))
+def test_window_attention_units_in_turns(case):
+    """Whole (sequence, key head) units to each XCD, their blocks in turns, with and without ranges of keys."""
+    O.check_attention(ops, gpu, case, seed=6)
+
+
 @pytest.mark.parametrize("name", ["both_sides", "token_grouped", "fp32_both_sides"])
 def test_window_attention_sharp_scores(name):
     """Scores up to a few hundred: one key carries a row, and the running maximum moves by more than the type's range."""
