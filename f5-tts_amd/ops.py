@@ -45,12 +45,14 @@ def _tensor(name: str, t: torch.Tensor, dtype: Optional[torch.dtype] = None, dev
         raise ValueError(f"{name} requires a gradient: the operators are for inference (use torch.no_grad())")
 
 
-def _lengths(name: str, t: Optional[torch.Tensor], like: torch.Tensor) -> Optional[torch.Tensor]:
+def _lengths(name: str, t: Optional[torch.Tensor], like: torch.Tensor, most: int) -> Optional[torch.Tensor]:
     if t is None:
         return None
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64) or t.shape != like.shape[:1] or t.device != like.device:
         raise ValueError(f"{name}: an int32 or int64 tensor of [batch] on {like.device} is expected")
-    return t.to(torch.int32).contiguous()
+    if t.dtype == torch.int64:
+        t = t.clamp(0, most).to(torch.int32)  # (the kernels clamp 32-bit lengths; narrowed first, 2^32 + 1 would be 1)
+    return t.contiguous()
 
 
 def _pack(layout: struct.Struct, fields) -> bytes:
@@ -173,7 +175,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}: heads and head_dim must be positive")
     if align not in _ALIGN:
         raise ValueError(f"align {align!r}: 'start' or 'end' is expected")
-    kv_len, q_len = _lengths("kv_len", kv_len, q), _lengths("q_len", q_len, q)
+    kv_len, q_len = _lengths("kv_len", kv_len, q, kshape[1]), _lengths("q_len", q_len, q, n)
     left, right = window
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_len is None else torch.zeros(shape, dtype=dtype, device=where)

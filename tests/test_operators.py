@@ -202,6 +202,22 @@ def test_window_attention_of_huge_scores_on_the_shim(host):
 
 
 @shim
+def test_lengths_are_clamped_whatever_their_type_on_the_shim(host):
+    q, k, v, kw = O.attention_inputs(O.ATTENTION["chunk"])
+    kw.pop("kv_len"), kw.pop("q_len")
+    want = host.window_attention(q, k, v, **kw)
+    tq, tk = q.shape[1], k.shape[1]
+    for lens in ([2 ** 63 - 1, 2 ** 32 + 1], [2 ** 31, 2 ** 32], [tk, tk + 1]):  # all of them, in 64 bits
+        assert torch.equal(host.window_attention(q, k, v, kv_len=torch.tensor(lens), q_len=torch.tensor(lens), **kw), want)
+    for low in (-1, -2 ** 32 + tq, -2 ** 63):  # none
+        n = torch.tensor([tq, low])
+        got = host.window_attention(q, k, v, q_len=n, **kw)
+        assert torch.equal(got[0], want[0]) and (got[1] == 0).all()
+        got = host.window_attention(q, k, v, kv_len=torch.tensor([tk, low]), **kw)
+        assert torch.equal(got[0], want[0]) and (got[1] == 0).all()
+
+
+@shim
 def test_axes_of_one_element_carry_any_stride_on_the_shim(host):
     x = torch.randn(128, generator=torch.Generator().manual_seed(4)).half()
     plain, odd = x.view(1, 1, 2, 64), x.as_strided((1, 1, 2, 64), (7, (1 << 40) + 3, 64, 1))
