@@ -184,6 +184,11 @@ class F5HipEngine:
         if rope_scaling not in binding.ROPE_SCALINGS:
             raise ValueError(f"rope_scaling {rope_scaling!r}: one of None, 'linear', 'ntk', 'yarn' is expected")
         left, right = (-1, -1) if window is None else (window, window) if isinstance(window, int) else window
+        # (the C structure's fields would take such numbers modulo 2^32 or 2^64)
+        for name, x, low, end in (("window", left, -1, 1 << 30), ("window", right, -1, 1 << 30), ("sinks", sinks, 0, 1 << 30),
+                                  ("rope_original_length", rope_original_length, 0, 1 << 63)):
+            if not low <= x < end:
+                raise ValueError(f"{name} = {x}: [{low}, {end}) is expected")
         cfg = binding.LongFormC(window_left=left, window_right=right, sinks=sinks, rope_scaling=binding.ROPE_SCALINGS[rope_scaling],
                                 rope_factor=rope_factor, rope_original_length=rope_original_length)
         with torch.cuda.device(self.device):

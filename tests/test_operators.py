@@ -72,6 +72,18 @@ def test_frequencies_refuse(kw):
         ops.rotary_frequencies(**kw)
 
 
+def test_long_form_refuses_numbers_past_its_fields():
+    """The engine's checks, before its library is called: 32-bit fields take 2^32 + 3 for 3."""
+    from f5_tts_amd.engine import F5HipEngine
+
+    eng = F5HipEngine.__new__(F5HipEngine)  # no library, no context: a call that got that far would raise AttributeError
+    for kw in (dict(window=1 << 32), dict(window=(1 << 32) + 3), dict(window=(5, 1 << 32)), dict(window=(-(1 << 32), 5)), dict(window=1 << 40),
+               dict(window=4, sinks=1 << 32), dict(window=4, sinks=-(1 << 32) + 1), dict(window=1 << 30), dict(window=(-2, 0)), dict(window=4, sinks=1 << 30),
+               dict(window=4, rope_scaling="yarn", rope_factor=2.0, rope_original_length=(1 << 64) + 2800)):
+        with pytest.raises(ValueError):
+            eng.set_long_form(**kw)
+
+
 # ---- refusals: before anything is launched ------------------------------------------------------------------------------------------------
 def q4(*shape, dtype=torch.float16):
     return torch.zeros(*shape, dtype=dtype)
