@@ -69,6 +69,8 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, *, scaling: Optional
     less than ``low`` (1) times over ``original_length`` positions are divided, those above ``high`` (32) kept, mixed between them)."""
     if scaling not in ROPE_SCALINGS:
         raise ValueError(f"scaling {scaling!r}: one of None, 'linear', 'ntk', 'yarn' is expected")
+    if not 0 < rot_dim <= 1 << 16 or not 0 <= original_length < 1 << 63:  # (the C arguments would take larger ones modulo 2^32 and 2^64)
+        raise ValueError(f"rot_dim {rot_dim} must be in [2, 65536], original_length {original_length} in [0, 2^63)")
     out, amplitude = (C.c_double * max(1, rot_dim // 2))(), C.c_double()
     lib = load_library()
     check(lib, None, lib.f5hip_rotary_frequencies(rot_dim, base, ROPE_SCALINGS[scaling], factor, original_length, low, high, out, C.byref(amplitude)))

@@ -84,6 +84,15 @@ def test_long_form_refuses_numbers_past_its_fields():
             eng.set_long_form(**kw)
 
 
+@pytest.mark.parametrize("kw", [dict(rot_dim=(1 << 32) + 2), dict(rot_dim=64, scaling="yarn", factor=2.0, original_length=(1 << 64) + 10)])
+def test_frequencies_refuse_numbers_past_their_types(kw, monkeypatch):
+    monkeypatch.setattr(ops.torch, "tensor", lambda *a, **k: pytest.fail("accepted"))  # (before the list of 2^31 numbers is made)
+    if kw["rot_dim"] > 1 << 16:
+        monkeypatch.setattr(ops, "load_library", lambda: pytest.fail("accepted"))
+    with pytest.raises(ValueError):
+        ops.rotary_frequencies(**kw)
+
+
 # ---- refusals: before anything is launched ------------------------------------------------------------------------------------------------
 def q4(*shape, dtype=torch.float16):
     return torch.zeros(*shape, dtype=dtype)
