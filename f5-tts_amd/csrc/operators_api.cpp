@@ -155,6 +155,7 @@ const char* scale_rotary_frequencies(double* f, int rot_dim, int scaling, double
       const double g = std::fmin(1.0, std::fmax(0.0, (r - low) / (high - low)));
       f[i] *= g + (1.0 - g) / factor;
     }
+    if (!std::isfinite(f[i])) return "rotary frequencies: the base and the factor give an infinite frequency";
   }
   *amplitude = scaling == F5HIP_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
   return nullptr;

@@ -93,6 +93,12 @@ def test_frequencies_refuse_numbers_past_their_types(kw, monkeypatch):
         ops.rotary_frequencies(**kw)
 
 
+@pytest.mark.parametrize("kw", [dict(scaling="linear", factor=1e-310), dict(scaling="ntk", factor=1e-320)])
+def test_infinite_frequencies_are_refused(kw):
+    with pytest.raises(ValueError, match="infinite"):
+        ops.rotary_frequencies(64, **kw)
+
+
 # ---- refusals: before anything is launched ------------------------------------------------------------------------------------------------
 def q4(*shape, dtype=torch.float16):
     return torch.zeros(*shape, dtype=dtype)
