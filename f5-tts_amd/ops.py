@@ -41,6 +41,10 @@ def _tensor(name: str, t: torch.Tensor, dtype: Optional[torch.dtype] = None, dev
             raise ValueError(f"{name}: {t.dtype} is not one of float32, float16, bfloat16")
     elif t.dtype != dtype or t.device != device:
         raise ValueError(f"{name}: {t.dtype} on {t.device}, the first tensor is {dtype} on {device}")
+    _inference(name, t)
+
+
+def _inference(name: str, t: torch.Tensor) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the operators are for inference (use torch.no_grad())")
 
@@ -92,6 +96,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
         raise ValueError(f"layout {layout!r}: 'interleaved' or 'half' is expected")
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != where:
         raise ValueError(f"inv_freq: a float64 vector on {where} is expected (rotary_frequencies)")
+    _inference("inv_freq", inv_freq)
     inv_freq = inv_freq.contiguous()
     b, n, h, d = shape
     hk = 0

@@ -150,6 +150,16 @@ def test_outputs_that_overlap_are_refused(host):
             host.window_attention(*qkv, out=qkv[i])
 
 
+def test_frequencies_that_require_a_gradient_are_refused(host):
+    x, f = q4(1, 4, 2, 64), O.frequencies(64).requires_grad_()
+    for layout in ("interleaved", "half"):
+        with pytest.raises(ValueError, match="gradient"):
+            host.rotary(x, None, f, layout=layout)
+    with torch.no_grad():
+        host.rotary(x, None, f)
+    host.rotary(x, None, f.detach())
+
+
 def test_numbers_past_fp32_are_refused(host):
     x = q4(1, 4, 2, 64)
     with pytest.raises(ValueError):
