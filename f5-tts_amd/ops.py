@@ -5,7 +5,7 @@ They are what the sampler runs in its blocks after ``F5HipEngine.set_long_form``
 fp32, fp16 or bf16, on the current stream of their device.  The reference calls ``apply_rotary_pos_emb`` and
 ``F.scaled_dot_product_attention`` in these places (``src/f5_tts/model/modules.py:498-520``).  Nothing is kept between calls: outputs and
 workspaces come from torch's allocator on the calling stream, so calls can be captured into graphs and run side by side.  Inference only:
-an input that requires a gradient is refused.
+an input that requires a gradient or carries a tangent is refused.
 """
 from __future__ import annotations
 
@@ -14,6 +14,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from .binding import ROPE_SCALINGS, F5HipError, check, load_library
 
@@ -47,6 +48,8 @@ def _tensor(name: str, t: torch.Tensor, dtype: Optional[torch.dtype] = None, dev
 def _inference(name: str, t: torch.Tensor) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the operators are for inference (use torch.no_grad())")
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:  # (-1: no dual level is open)
+        raise ValueError(f"{name} carries a tangent of forward-mode differentiation: the operators are for inference (use its primal)")
 
 
 def _lengths(name: str, t: Optional[torch.Tensor], like: torch.Tensor, most: int) -> Optional[torch.Tensor]:

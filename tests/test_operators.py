@@ -160,6 +160,27 @@ def test_frequencies_that_require_a_gradient_are_refused(host):
     host.rotary(x, None, f.detach())
 
 
+def test_forward_mode_tangents_are_refused(host):
+    from torch.autograd import forward_ad as fw
+
+    x, f = q4(1, 4, 2, 64, dtype=torch.float32), O.frequencies(64)
+    with fw.dual_level():
+        dual, turn = fw.make_dual(x, torch.ones_like(x)), fw.make_dual(f, torch.ones_like(f))
+        for args in ((dual, None, f), (x, dual, f), (x, None, turn)):
+            with pytest.raises(ValueError, match="tangent"):
+                host.rotary(*args)
+        with pytest.raises(ValueError, match="tangent"):
+            host.rotary(x, None, f, out=(dual, None))
+        for i in range(3):
+            qkv = [x, x, x]
+            qkv[i] = dual
+            with pytest.raises(ValueError, match="tangent"):
+                host.window_attention(*qkv)
+        with pytest.raises(ValueError, match="tangent"):
+            host.window_attention(x, x, x, out=fw.make_dual(torch.zeros_like(x), torch.ones_like(x)))
+        host.window_attention(x, x, host.rotary(fw.unpack_dual(dual).primal, None, f)[0])
+
+
 def test_numbers_past_fp32_are_refused(host):
     x = q4(1, 4, 2, 64)
     with pytest.raises(ValueError):
