@@ -100,6 +100,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != where:
         raise ValueError(f"inv_freq: a float64 vector on {where} is expected (rotary_frequencies)")
     _inference("inv_freq", inv_freq)
+    if isinstance(amplitude, torch.Tensor):
+        _inference("amplitude", amplitude)
     inv_freq = inv_freq.contiguous()
     b, n, h, d = shape
     hk = 0
@@ -183,6 +185,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}, v {tuple(v.shape)}: batch and head_dim must agree, k and v in all axes")
     if d == 0 or h == 0 or kshape[2] == 0:
         raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}: heads and head_dim must be positive")
+    if isinstance(scale, torch.Tensor):
+        _inference("scale", scale)
     if align not in _ALIGN:
         raise ValueError(f"align {align!r}: 'start' or 'end' is expected")
     kv_len, q_len = _lengths("kv_len", kv_len, q, kshape[1]), _lengths("q_len", q_len, q, n)

@@ -160,6 +160,16 @@ def test_frequencies_that_require_a_gradient_are_refused(host):
     host.rotary(x, None, f.detach())
 
 
+def test_numbers_that_require_a_gradient_are_refused(host):
+    x, f, learned = q4(1, 4, 2, 64), O.frequencies(64), torch.tensor(0.5, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        host.rotary(x, None, f, amplitude=learned)
+    with pytest.raises(ValueError, match="gradient"):
+        host.window_attention(x, x, x, scale=learned)
+    host.rotary(x, None, f, amplitude=learned.detach())
+    host.window_attention(x, x, x, scale=learned.detach())
+
+
 def test_forward_mode_tangents_are_refused(host):
     from torch.autograd import forward_ad as fw
 
