@@ -62,6 +62,10 @@ def _lengths(name: str, t: Optional[torch.Tensor], like: torch.Tensor, most: int
     return t.contiguous()
 
 
+# a tensor, or an iterable of them, was written behind torch's back: an operation that saved it for its backward pass has to notice
+_written = torch.autograd.graph.increment_version
+
+
 def _pack(layout: struct.Struct, fields) -> bytes:
     try:
         return layout.pack(*fields)
@@ -149,6 +153,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
     status = lib.f5hip_rotary(args, device, stream)
     if status:
         check(lib, None, status)
+    if out is not None:
+        _written(q_out if k is None else out)
     return q_out, k_out
 
 
@@ -191,6 +197,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         raise ValueError(f"align {align!r}: 'start' or 'end' is expected")
     kv_len, q_len = _lengths("kv_len", kv_len, q, kshape[1]), _lengths("q_len", q_len, q, n)
     left, right = window
+    given = out
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_len is None else torch.zeros(shape, dtype=dtype, device=where)
     else:
@@ -218,4 +225,6 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     status = lib.f5hip_window_attention(args, device, stream)
     if status:
         check(lib, None, status)
+    if given is not None:
+        _written(out)
     return out

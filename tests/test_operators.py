@@ -286,6 +286,23 @@ def test_lengths_are_clamped_whatever_their_type_on_the_shim(host):
 
 
 @shim
+def test_writes_are_noticed_by_autograd_on_the_shim(host):
+    f, x = O.frequencies(64), torch.randn(2, 4, 2, 64, generator=torch.Generator().manual_seed(2))
+    calls = [lambda y: host.rotary(y, None, f, out=(y, None)), lambda y: host.rotary(x, x, f, out=(torch.empty_like(x), y)),
+             lambda y: host.window_attention(x, x, x, out=y), lambda y: host.rotary(x, y[:, :, :1], f, out=(torch.empty_like(x), y[:, :, :1]))]
+    for call in calls:
+        y, w = x.clone(), torch.ones_like(x, requires_grad=True)
+        loss = (w * y).sum()  # saves y
+        call(y)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():  # such tensors count no versions
+        y = x.clone()
+        host.rotary(y, y.clone(), f, out=(y, torch.empty_like(y)))
+        host.window_attention(y, y, y, out=torch.empty_like(y))
+
+
+@shim
 def test_axes_of_one_element_carry_any_stride_on_the_shim(host):
     x = torch.randn(128, generator=torch.Generator().manual_seed(4)).half()
     plain, odd = x.view(1, 1, 2, 64), x.as_strided((1, 1, 2, 64), (7, (1 << 40) + 3, 64, 1))
