@@ -154,7 +154,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
     if status:
         check(lib, None, status)
     if out is not None:
-        _written(q_out if k is None else out)
+        _written(q_out if k is None else (q_out, k_out))
     return q_out, k_out
 
 
