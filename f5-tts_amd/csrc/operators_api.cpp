@@ -1,4 +1,5 @@
 // operators_api.cpp — entry points of the operators (include/f5hip.h, "operators"): argument checks, device guard, per-thread error text.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 
@@ -42,13 +43,74 @@ f5hip_window_attention_args plain(const f5hip_window_attention_args& args) {
   drop_idle_strides(a.v_stride, a.batch, a.kv_tokens, a.kv_heads);
   return a;
 }
-// an output that starts where its input does has the input's strides
-bool in_place_or_apart(const void* in, const void* out, const int64_t (&si)[3], const int64_t (&so)[3], const int64_t (&ext)[3]) {
-  for (int i = 0; i < 3; ++i)
-    if (in == out && ext[i] > 1 && si[i] != so[i]) return false;
-  return true;
+// a buffer as runs of `run` bytes: at `base` plus any multiples x_i < n_i of the strides, in bytes
+struct Runs {
+  const void* base;
+  int64_t run, n[3], stride[3];
+  Runs(const void* p, int64_t bytes) : base(p), run(p ? bytes : 0), n{1, 1, 1}, stride{0, 0, 0} {}
+  Runs(const void* p, int dim, int eb, const int64_t (&st)[3], const int64_t (&ext)[3]) : Runs(p, (int64_t)dim * eb) {
+    for (int i = 0; i < 3; ++i) {
+      if (ext[i] < 1) run = 0;  // no element
+      if (ext[i] > 1 && st[i] > 0) { n[i] = ext[i]; stride[i] = st[i] * eb; }
+    }
+  }
+  uintptr_t begin() const { return reinterpret_cast<uintptr_t>(base); }
+  uintptr_t end() const { return begin() + (uintptr_t)(run + (n[0] - 1) * stride[0] + (n[1] - 1) * stride[1] + (n[2] - 1) * stride[2]); }
+};
+// Is there a sum of c_i s_i, low_i <= c_i <= high_i, between `above` and `below` — with `moved`, one whose c_i are not all 0?  Strides in falling order,
+// so what the smaller ones reach leaves few c_i to try: for views of one buffer a handful.  Strides that leave more than 2^16 are taken for a yes.
+struct Reach {
+  int dims = 0, left = 1 << 16;
+  int64_t s[6], low[6], high[6];
+  void add(int64_t stride, int64_t from, int64_t to) {
+    if (!stride) return;
+    int i = 0;
+    while (i < dims && s[i] > stride) ++i;
+    if (i == dims || s[i] != stride) {
+      for (int j = dims++; j > i; --j) { s[j] = s[j - 1]; low[j] = low[j - 1]; high[j] = high[j - 1]; }
+      s[i] = stride;
+      low[i] = high[i] = 0;
+    }
+    low[i] += from;
+    high[i] += to;
+  }
+  bool between(int64_t above, int64_t below, bool moved, int i = 0) {
+    if (i == dims) return above < 0 && 0 < below && moved;
+    int64_t least = 0, most = 0;
+    for (int j = i + 1; j < dims; ++j) { least += low[j] * s[j]; most += high[j] * s[j]; }
+    // the c with above < c s + (something in [least, most]) < below
+    const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+    const int64_t from = std::max(low[i], floor_div(above - most, s[i]) + 1), to = std::min(high[i], -floor_div(least - below, s[i]) - 1);
+    for (int64_t c = from; c <= to; ++c)
+      if (--left < 0 || between(above - c * s[i], below - c * s[i], moved || c != 0, i + 1)) return true;
+    return false;
+  }
+};
+bool share_memory(const Runs& a, const Runs& b) {
+  if (!a.run || !b.run || a.end() <= b.begin() || b.end() <= a.begin()) return false;
+  Reach r;
+  for (int i = 0; i < 3; ++i) {
+    r.add(a.stride[i], 0, a.n[i] - 1);
+    r.add(b.stride[i], 1 - b.n[i], 0);
+  }
+  const int64_t apart = (int64_t)(b.begin() - a.begin());
+  return r.between(apart - a.run, apart + b.run, true);
 }
-bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+bool elements_overlap(const Runs& a) {
+  Reach r;
+  for (int i = 0; i < 3; ++i) r.add(a.stride[i], 1 - a.n[i], a.n[i] - 1);
+  int64_t inner = a.run;  // each stride past what the smaller ones reach (two equal ones overlap): the ordinary tensor
+  bool nested = a.run > 0;
+  for (int i = r.dims - 1; i >= 0; --i) {
+    nested = nested && r.s[i] >= inner;
+    inner += r.high[i] * r.s[i];
+  }
+  int axes = 0;
+  for (int64_t st : a.stride) axes += st > 0;
+  return a.run > 0 && (axes != r.dims || (!nested && r.between(-a.run, a.run, false)));
+}
+bool same_strides(const int64_t (&x)[3], const int64_t (&y)[3]) { return x[0] == y[0] && x[1] == y[1] && x[2] == y[2]; }
+bool aligned(const void* p, int a) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(a - 1)) == 0; }
 
 // the calling thread's device while an operator launches, restored on every path
 struct DeviceGuard {
@@ -92,17 +154,26 @@ const char* check_rotary(const f5hip_rotary_args& a) {
   if (!std::isfinite(a.amplitude)) return "rotary: amplitude must be finite";
   if (a.batch == 0 || a.tokens == 0) return nullptr;  // nothing to do: empty tensors have no pointers
   if (!a.q || !a.q_out || !a.inv_freq || (a.heads_k && (!a.k || !a.k_out))) return "rotary: null pointer";
-  const uintptr_t eb = (uintptr_t)elt_bytes(a.dtype);
+  const int eb = elt_bytes(a.dtype);
   if (!aligned(a.q, eb) || !aligned(a.q_out, eb) || (a.heads_k && (!aligned(a.k, eb) || !aligned(a.k_out, eb)))) return "rotary: pointer not aligned to its elements";
   if (!aligned(a.inv_freq, 8) || (a.positions && !aligned(a.positions, 8))) return "rotary: inv_freq / positions not aligned to 8 bytes";
   const int64_t eq[3] = {a.batch, a.tokens, a.heads_q}, ek[3] = {a.batch, a.tokens, a.heads_k};
   if (!strides_ok(a.q_stride, eq, false) || !strides_ok(a.q_out_stride, eq, true) ||
       (a.heads_k && (!strides_ok(a.k_stride, ek, false) || !strides_ok(a.k_out_stride, ek, true))))
     return "rotary: strides must lie in [0, 2^40], an output's must not be 0";
-  if (!in_place_or_apart(a.q, a.q_out, a.q_stride, a.q_out_stride, eq) ||
-      (a.heads_k && (!in_place_or_apart(a.k, a.k_out, a.k_stride, a.k_out_stride, ek) || a.q_out == a.k || a.k_out == a.q || a.q_out == a.k_out)))
-    return "rotary: an output may be its own input with the same strides, or memory of its own";
   if (a.position_stride < 0 || a.position_stride > (int64_t(1) << 40)) return "rotary: position_stride must lie in [0, 2^40]";
+  const Runs q(a.q, a.head_dim, eb, a.q_stride, eq), qo(a.q_out, a.head_dim, eb, a.q_out_stride, eq);
+  const Runs k(a.heads_k ? a.k : nullptr, a.head_dim, eb, a.k_stride, ek), ko(a.heads_k ? a.k_out : nullptr, a.head_dim, eb, a.k_out_stride, ek);
+  if (elements_overlap(qo) || elements_overlap(ko)) return "rotary: an output's elements must not overlap";
+  // (strides of idle axes have been dropped: equal ones are the same view)
+  const bool q_in_place = a.q == a.q_out && same_strides(a.q_stride, a.q_out_stride), k_in_place = a.k == a.k_out && same_strides(a.k_stride, a.k_out_stride);
+  if ((!q_in_place && share_memory(qo, q)) || (!k_in_place && share_memory(ko, k)) || share_memory(qo, k) || share_memory(ko, q) || share_memory(qo, ko))
+    return "rotary: an output may be its own input with the same strides, or memory of its own";
+  const Runs freq(a.inv_freq, a.rot_dim / 2 * 8);
+  Runs at(a.positions, (int64_t)a.tokens * 8);
+  if (a.position_stride > 0) { at.n[0] = a.batch; at.stride[0] = a.position_stride * 8; }
+  for (const Runs* in : {&freq, (const Runs*)&at})
+    if (share_memory(qo, *in) || share_memory(ko, *in)) return "rotary: an output must share no memory with inv_freq and positions";
   return nullptr;
 }
 
@@ -123,7 +194,6 @@ const char* check_window_attention(const f5hip_window_attention_args& a) {
   if ((int64_t)a.batch * a.heads * a.q_tokens >= lim) return "window attention: batch * heads * q_tokens must be below 2^30";
   if (a.batch == 0 || a.q_tokens == 0) return nullptr;
   if (!a.q || !a.out || (a.kv_tokens && (!a.k || !a.v))) return "window attention: null pointer";
-  if (a.out == a.q || (a.kv_tokens && (a.out == a.k || a.out == a.v))) return "window attention: out must share no memory with q, k and v";
   if (!aligned(a.q, 16) || !aligned(a.k, 16) || !aligned(a.v, 16) || !aligned(a.out, 16)) return "window attention: pointers must be aligned to 16 bytes";
   if (!aligned(a.kv_len, 4) || !aligned(a.q_len, 4)) return "window attention: lengths must be aligned to 4 bytes";
   const int64_t eq[3] = {a.batch, a.q_tokens, a.heads}, ek[3] = {a.batch, a.kv_tokens, a.kv_heads};
@@ -135,6 +205,12 @@ const char* check_window_attention(const f5hip_window_attention_args& a) {
       if (((*st)[i] * eb) % 16) return "window attention: strides must be whole multiples of 16 bytes";
   // a 64-key tile is addressed with 31-bit byte offsets from its first key
   if (a.k_stride[1] * eb * 64 >= (int64_t(1) << 31) || a.v_stride[1] * eb * 64 >= (int64_t(1) << 31)) return "window attention: 64 key rows must span less than 2 GiB";
+  const Runs out(a.out, a.head_dim, eb, a.out_stride, eq);
+  if (elements_overlap(out)) return "window attention: out's elements must not overlap";
+  const Runs q(a.q, a.head_dim, eb, a.q_stride, eq), k(a.k, a.head_dim, eb, a.k_stride, ek), v(a.v, a.head_dim, eb, a.v_stride, ek);
+  const Runs kv_len(a.kv_len, (int64_t)a.batch * 4), q_len(a.q_len, (int64_t)a.batch * 4);
+  for (const Runs* in : {&q, &k, &v, &kv_len, &q_len})
+    if (share_memory(out, *in)) return "window attention: out must share no memory with q, k and v, nor with the lengths";
   return nullptr;
 }
 

@@ -96,7 +96,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
     copied.  ``layout``: pairs are columns ``(2i, 2i + 1)`` ("interleaved") or ``(i, i + R / 2)`` ("half").  ``positions``: int64
     ``[batch, tokens]`` or ``[tokens]``; without them token t stands at ``offset + t``.  ``rot_heads``: only the first so many heads of q and of
     k rotate (the reference's ``pe_attn_head``).  ``inverse`` turns back (with amplitude 1 the inverse; in any case the operator's gradient).
-    ``out``: ``(q', k')`` to write to — the inputs themselves, or tensors that share no memory with them."""
+    ``out``: ``(q', k')`` to write to — the inputs themselves, or tensors that share no element with them (other columns of one buffer do not)."""
     _tensor("q", q)
     dtype, where, shape = q.dtype, q.device, q.shape
     if layout not in _LAYOUTS:
@@ -180,7 +180,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     no bound on that side; ``right = 0``: causal) and, of the first ``sinks`` keys, all that ``right`` allows.  A query that sees no key gives
     zeros.  ``kv_len``, ``q_len``: valid keys and queries of each sequence; output rows behind ``q_len`` are zero, or left as they were in
     ``out``.  ``scale``: 1 / sqrt(D) by default.  D: a multiple of 8 (fp32: 4) up to 128.  Keys and values that no query sees may hold
-    anything, a value that some query sees has to be finite for the others' sake; tensors whose rows are not aligned to 16 bytes are copied first.  ``out`` shares no memory with q, k and v."""
+    anything, a value that some query sees has to be finite for the others' sake; tensors whose rows are not aligned to 16 bytes are copied first.  ``out`` shares no element with q, k and v."""
     _tensor("q", q)
     dtype, where, shape = q.dtype, q.device, q.shape
     _tensor("k", k, dtype, where)

@@ -307,7 +307,8 @@ int f5hip_rotary_frequencies(int rot_dim, double base, int scaling, double facto
  * p inv_freq[i] (inverse != 0: minus the angle; the gradient of the operator).  The angle and its reduction are taken in 64 bits — exact to
  * fp32 rounding for |p| up to 2^31 and beyond —, the rotation in fp32, and each output is rounded once.  Columns >= rot_dim and, where rot_heads >= 0,
  * heads >= rot_heads (of q and of k: the reference's pe_attn_head, modules.py:504-509) are copied.
- * An output may be its input (same pointer, same strides); any other overlap is not allowed.  heads_k = 0: q alone. */
+ * An output may be its input (same pointer, same strides); any other element that an output shares with a buffer of the call, or has twice, is
+ * refused (views whose elements lie between each other's are none of these).  heads_k = 0: q alone. */
 typedef struct f5hip_rotary_args {
   int32_t dtype, layout, inverse, rot_dim;
   int32_t batch, tokens, heads_q, heads_k, head_dim, rot_heads;
@@ -330,7 +331,7 @@ int f5hip_rotary(const f5hip_rotary_args* args, int device, void* stream);
  * are fp32; with 16-bit types the weights are rounded to that type for the product with v (the softmax sum is that of the rounded weights).
  * Scores have to stay below 2^22 in magnitude (an fp32 dot product of that size has lost the differences a softmax reads).
  * fp32 tensors are multiplied as three bf16 pieces a number, six products of nine: fp32 accuracy for finite numbers; an infinity that is seen gives
- * NaN.  `out` shares no memory with q, k and v.
+ * NaN.  `out` shares no element with q, k, v and the lengths, and has none twice: refused (it may lie between their rows or heads).
  *   kv_len, q_len   device int32 [batch] or NULL (kv_tokens / q_tokens), clamped into [0, kv_tokens] / [0, q_tokens].  Output rows
  *                   i >= q_len[b] are left as they were.  Keys at and past kv_len[b] and keys in front of every query's window are not
  *                   read, whatever they hold; a v row that SOME query of the call sees has to be finite for the others' sake.

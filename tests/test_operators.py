@@ -3,6 +3,7 @@ host shim (tests/hipemu) against the 64-bit restatement in tests/operators_oracl
 import ctypes as C
 import math
 import os
+import random
 import sys
 
 import pytest
@@ -148,6 +149,68 @@ def test_outputs_that_overlap_are_refused(host):
         qkv = [q4(2, 4, 2, 64) for _ in range(3)]
         with pytest.raises(ValueError, match="no memory"):
             host.window_attention(*qkv, out=qkv[i])
+
+
+def test_outputs_that_overlap_in_part_are_refused(host):
+    f = O.frequencies(64)
+    buf = q4(2, 6, 12, 64)  # q | k | v | o, three heads each
+    q, k, v, o = (buf[:, :, 3 * i:3 * i + 3] for i in range(4))
+    host.rotary(q, k, f, out=(q, k))
+    host.rotary(q, k, f, out=(v, o))
+    host.window_attention(q, k, v, out=o)
+    host.window_attention(q[:, :2], k, v, out=q[:, 2:4])  # rows between
+    one_head_on = buf[:, :, 1:4]
+    for out in ((one_head_on, v), (v, one_head_on), (v, buf[:, :, 7:10]), (buf[:, :, 5:8], o)):
+        with pytest.raises(ValueError, match="own input"):
+            host.rotary(q, k, f, out=out)
+    with pytest.raises(ValueError, match="own input"):
+        host.rotary(buf.flatten()[:6 * 192].view(1, 6, 3, 64), None, f, out=(buf.flatten()[1:6 * 192 + 1].view(1, 6, 3, 64), None))
+    for out in (one_head_on, buf[:, :, 2:5], buf[:, :, 8:11], buf.flatten()[8 * 64:8 * 64 + 2 * 6 * 192].view(2, 6, 3, 64)):
+        with pytest.raises(ValueError, match="no memory"):
+            host.window_attention(q, k, v, out=out)
+    lens = buf.view(torch.int32)[0, 0, 11, :2]
+    for kw in (dict(kv_len=lens), dict(q_len=lens)):
+        with pytest.raises(ValueError, match="lengths"):
+            host.window_attention(q, k, v, out=o, **kw)
+    wide = torch.zeros(4 * 64, dtype=torch.float64)
+    y = wide.view(torch.float32)
+    with pytest.raises(ValueError, match="inv_freq"):
+        host.rotary(torch.zeros(1, 1, 1, 64), None, wide[:32], out=(y[32:96].view(1, 1, 1, 64), None))
+    with pytest.raises(ValueError, match="positions"):
+        host.rotary(torch.zeros(2, 4, 1, 64), None, f, positions=y.view(torch.int64)[-8:].view(2, 4), out=(y[:512].view(2, 4, 1, 64), None))
+    with pytest.raises(ValueError, match="elements"):
+        host.rotary(torch.zeros(2, 4, 1, 64), None, f, out=(y.as_strided((2, 4, 1, 64), (128, 32, 64, 1)), None))
+    with pytest.raises(ValueError, match="elements"):
+        host.window_attention(q, k, v, out=torch.zeros(2, 6, 3, 64).half().as_strided((2, 6, 3, 64), (64, 128, 64, 1)))
+
+
+@shim
+def test_overlaps_are_found_exactly_on_the_shim(host):
+    """Random views of one buffer, the refusal against the sets of their elements."""
+    rng, f = random.Random(5), O.frequencies(4)
+    said = {True: 0, False: 0}
+    for _ in range(3000):
+        shape = (rng.randint(1, 3), rng.randint(1, 4), rng.randint(1, 3), 4)
+        buf = torch.zeros(700)
+        views, cells = [], []
+        for _ in range(2):
+            st = [rng.choice([0, 1, 2, 3, 4, 5, 8, 12, 13, 16, 24, 36, 48, 49]) if m > 1 else 0 for m in shape[:3]]
+            at = rng.choice([0, 4, 12, 17, rng.randint(0, 200)])
+            views.append(buf.as_strided(shape, (*st, 1), at))
+            cells.append(torch.arange(700).as_strided(shape, (*st, 1), at).flatten().tolist())
+        if rng.random() < 0.2:
+            views[1], cells[1] = views[0], cells[0]
+        (x, y), (a, b) = views, cells
+        wrong = len(set(b)) < len(b) or (bool(set(a) & set(b)) and x is not y and not (x.data_ptr() == y.data_ptr() and x.stride() == y.stride()))
+        try:
+            host.rotary(x, None, f, out=(y, None))
+            refused = False
+        except ValueError as e:
+            refused = True
+            assert "output" in str(e), e
+        assert refused == wrong, (shape, x.stride(), y.stride(), x.storage_offset(), y.storage_offset())
+        said[wrong] += 1
+    assert min(said.values()) > 300
 
 
 def test_frequencies_that_require_a_gradient_are_refused(host):
