@@ -13,13 +13,15 @@ int f5hip_set_thread_error(int code, const char* text);  // api.cpp: the text f5
 namespace {
 int elt_bytes(int dtype) { return dtype == F5HIP_T_FP32 ? 4 : 2; }
 
-// |any element offset| of a [batch, tokens, heads, dim] tensor stays far below 2^63, so the kernels' 64-bit offsets cannot wrap
+// every element's offset in bytes stays far below 2^63, so 64-bit offsets cannot wrap (no address space has more than 2^57)
 bool strides_ok(const int64_t (&st)[3], const int64_t (&ext)[3], bool output) {
+  __int128 span = 0;
   for (int i = 0; i < 3; ++i) {
     if (st[i] < 0 || st[i] > (int64_t(1) << 40)) return false;
     if (output && st[i] == 0 && ext[i] > 1) return false;
+    if (ext[i] > 1) span += (__int128)(ext[i] - 1) * st[i];
   }
-  return true;
+  return span < (int64_t(1) << 55);
 }
 // an axis of at most one element may carry any stride: none
 void drop_idle_strides(int64_t (&st)[3], int64_t batch, int64_t tokens, int64_t heads) {
@@ -160,8 +162,11 @@ const char* check_rotary(const f5hip_rotary_args& a) {
   const int64_t eq[3] = {a.batch, a.tokens, a.heads_q}, ek[3] = {a.batch, a.tokens, a.heads_k};
   if (!strides_ok(a.q_stride, eq, false) || !strides_ok(a.q_out_stride, eq, true) ||
       (a.heads_k && (!strides_ok(a.k_stride, ek, false) || !strides_ok(a.k_out_stride, ek, true))))
-    return "rotary: strides must lie in [0, 2^40], an output's must not be 0";
-  if (a.position_stride < 0 || a.position_stride > (int64_t(1) << 40)) return "rotary: position_stride must lie in [0, 2^40]";
+    return "rotary: strides must lie in [0, 2^40] and a tensor must span less than 2^55 elements, an output's strides must not be 0";
+  if (a.position_stride < 0 || a.position_stride > (int64_t(1) << 40) || (a.positions && (__int128)a.position_stride * a.batch >= int64_t(1) << 55))
+    return "rotary: position_stride must lie in [0, 2^40] and the positions must span less than 2^55 elements";
+  // (the last token's position is worked out in 64 bits)
+  if (!a.positions && a.first > INT64_MAX - a.tokens) return "rotary: first + tokens must stay below 2^63";
   const Runs q(a.q, a.head_dim, eb, a.q_stride, eq), qo(a.q_out, a.head_dim, eb, a.q_out_stride, eq);
   const Runs k(a.heads_k ? a.k : nullptr, a.head_dim, eb, a.k_stride, ek), ko(a.heads_k ? a.k_out : nullptr, a.head_dim, eb, a.k_out_stride, ek);
   if (elements_overlap(qo) || elements_overlap(ko)) return "rotary: an output's elements must not overlap";
@@ -198,7 +203,7 @@ const char* check_window_attention(const f5hip_window_attention_args& a) {
   if (!aligned(a.kv_len, 4) || !aligned(a.q_len, 4)) return "window attention: lengths must be aligned to 4 bytes";
   const int64_t eq[3] = {a.batch, a.q_tokens, a.heads}, ek[3] = {a.batch, a.kv_tokens, a.kv_heads};
   if (!strides_ok(a.q_stride, eq, false) || !strides_ok(a.out_stride, eq, true) || !strides_ok(a.k_stride, ek, false) || !strides_ok(a.v_stride, ek, false))
-    return "window attention: strides must lie in [0, 2^40], the output's must not be 0";
+    return "window attention: strides must lie in [0, 2^40] and a tensor must span less than 2^55 elements, the output's strides must not be 0";
   const int64_t (*all[4])[3] = {&a.q_stride, &a.k_stride, &a.v_stride, &a.out_stride};
   for (auto* st : all)
     for (int i = 0; i < 3; ++i)

@@ -262,6 +262,39 @@ def test_numbers_past_fp32_are_refused(host):
         host.window_attention(x, x, x, scale=1e39)
 
 
+class RotaryC(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "layout", "inverse", "rot_dim", "batch", "tokens", "heads_q", "heads_k", "head_dim", "rot_heads")] + \
+        [("amplitude", C.c_float)] + [(n, C.c_void_p) for n in ("q", "k", "q_out", "k_out")] + \
+        [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "q_out_stride", "k_out_stride")] + \
+        [("inv_freq", C.c_void_p), ("positions", C.c_void_p), ("position_stride", C.c_int64), ("first", C.c_int64)]
+
+
+def rotary_c(**kw):
+    """f5hip_rotary_args of 2 x 4 tokens of 2 heads of 64, fp16; the pointers are nobody's memory: for calls that are refused."""
+    a = RotaryC(dtype=1, rot_dim=64, batch=2, tokens=4, heads_q=2, head_dim=64, rot_heads=-1, amplitude=1.0, q=1 << 40, q_out=1 << 41, inv_freq=1 << 42)
+    a.q_stride[:] = a.q_out_stride[:] = [512, 128, 64]
+    for name, x in kw.items():
+        if isinstance(x, list):
+            getattr(a, name)[:] = x
+        else:
+            setattr(a, name, x)
+    return a
+
+
+def refusal(lib, a):
+    code = lib.f5hip_rotary(C.addressof(a), 0, None)
+    return code, lib.f5hip_last_error(None).decode()
+
+
+def test_rotary_refuses_offsets_past_64_bits(operators_emu_lib):
+    """Sizes and strides that are each within their limits, products that are not; nothing is launched."""
+    for kw, why in ((dict(tokens=1 << 30, q_stride=[0, 1 << 40, 64]), "span"), (dict(batch=1 << 20, q_out_stride=[1 << 40, 128, 64]), "span"),
+                    (dict(batch=1 << 20, positions=1 << 43, position_stride=1 << 40, q_stride=[0, 128, 64]), "positions"),
+                    (dict(first=(1 << 63) - 4), "first"), (dict(first=(1 << 63) - 1), "first")):
+        code, text = refusal(operators_emu_lib, rotary_c(**kw))
+        assert code == 1 and why in text, (kw, text)
+
+
 def test_c_entries_refuse_null_and_say_why():
     lib = binding.load_library()
     assert lib.f5hip_rotary(None, 0, None) == 1 and b"null" in lib.f5hip_last_error(None)
