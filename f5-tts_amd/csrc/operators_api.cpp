@@ -179,6 +179,7 @@ const char* check_rotary(const f5hip_rotary_args& a) {
   if (a.position_stride > 0) { at.n[0] = a.batch; at.stride[0] = a.position_stride * 8; }
   for (const Runs* in : {&freq, (const Runs*)&at})
     if (share_memory(qo, *in) || share_memory(ko, *in)) return "rotary: an output must share no memory with inv_freq and positions";
+  if (rotary_threads(a) > ROTARY_THREADS) return "rotary: a sequence of more than 2^31 pieces (of up to 16 bytes, as alignment allows)";
   return nullptr;
 }
 

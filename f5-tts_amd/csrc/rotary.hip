@@ -135,53 +135,82 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   }
 }
 
-template <typename T, int VEC, bool TWO>
-hipError_t launch(RotaryArgs& r, int head_dim, hipStream_t s) {
-  r.npair = TWO ? r.rot / 2 / VEC : r.rot / VEC;
-  r.nitem = r.npair + (head_dim - r.rot) / VEC;
+// the pieces of a call and their threads
+struct Plan {
+  int vec, npair, nitem, hg;  // elements of a piece; pieces of a head that rotate, all of them; heads of a thread stand hg apart
+  bool two;                   // a thread's pairs are in two pieces
+  int per;                    // heads of a thread
+  int64_t threads;            // of a sequence
+};
+Plan plan_of(const f5hip_rotary_args& a) {
+  Plan p{};
+  // The widest piece (16 bytes at most) that divides the rotated columns (their half in the half layout), the columns behind them, every
+  // stride and every pointer.
+  const int eb = a.dtype == F5HIP_T_FP32 ? 4 : 2;
+  const bool half = a.layout == F5HIP_ROTARY_HALF;
+  const auto fits = [&](int v) {
+    if ((half ? a.rot_dim / 2 : a.rot_dim) % v || (a.head_dim - a.rot_dim) % v) return false;
+    for (int i = 0; i < 3; ++i)
+      if (a.q_stride[i] % v || a.q_out_stride[i] % v || (a.heads_k && (a.k_stride[i] % v || a.k_out_stride[i] % v))) return false;
+    uintptr_t p = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out);
+    if (a.heads_k) p |= reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.k_out);
+    return p % (uintptr_t)(v * eb) == 0;
+  };
+  p.vec = 16 / eb;
+  while (p.vec > 1 && !fits(p.vec)) p.vec /= 2;
+  p.two = half || p.vec == 1;
+  p.npair = p.two ? a.rot_dim / 2 / p.vec : a.rot_dim / p.vec;
+  p.nitem = p.npair + (a.head_dim - a.rot_dim) / p.vec;
   // Heads per thread: one until the call has half as many items as the chip holds threads (256 CUs x 2048), two above (4 x 8192 tokens of 40 heads of
   // 128: 134 us, with four heads and their registers 139 us, with one 135 us; 2 x 1406 tokens of 32 heads of 64: 6.6, 7.8, 7.6 us).
-  const int64_t items = (int64_t)r.batch * r.tokens * r.heads * r.nitem;
-  const int per = items < 256 * 1024 ? 1 : 2;
-  r.hg = (r.heads + per - 1) / per;
-  const int64_t threads = (int64_t)r.tokens * r.nitem * r.hg;
-  if (threads > 0x7fffff00) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)std::min(r.batch, 65535));
+  const int heads = a.heads_q + a.heads_k;
+  const int64_t items = (int64_t)a.batch * a.tokens * heads * p.nitem;
+  p.per = items < 256 * 1024 ? 1 : 2;
+  p.hg = (heads + p.per - 1) / p.per;
+  p.threads = (int64_t)a.tokens * p.nitem * p.hg;
+  return p;
+}
+
+template <typename T, int VEC, bool TWO>
+hipError_t launch(const RotaryArgs& r, const Plan& p, hipStream_t s) {
+  const dim3 grid((unsigned)((p.threads + 255) / 256), (unsigned)std::min(r.batch, 65535));
   // 256 threads touch at most 256 / slots + 2 tokens: 48 KiB for the largest head, under 17 KiB for the smallest
-  const int64_t slots = (int64_t)r.nitem * r.hg;
+  const int64_t slots = (int64_t)p.nitem * p.hg;
   const size_t lds = (size_t)(256 / slots + 2) * (r.rot / 2) * sizeof(float2);
-  if (per == 1) hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 1>), grid, dim3(256), lds, s, r);
+  if (p.per == 1) hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 1>), grid, dim3(256), lds, s, r);
   else hipLaunchKernelGGL((rotary_kernel<T, VEC, TWO, 2>), grid, dim3(256), lds, s, r);
   return hipGetLastError();
 }
 
 template <typename T, int VEC>
-hipError_t launch_layout(RotaryArgs& r, int head_dim, bool half, hipStream_t s) {
+hipError_t launch_layout(RotaryArgs& r, const Plan& p, bool half, hipStream_t s) {
   if (half) {
     r.step = VEC;
     r.off_b = r.rot / 2;
-    return launch<T, VEC, true>(r, head_dim, s);
+    return launch<T, VEC, true>(r, p, s);
   }
   if constexpr (VEC > 1) {
     r.step = VEC;
     r.off_b = 0;
-    return launch<T, VEC, false>(r, head_dim, s);
+    return launch<T, VEC, false>(r, p, s);
   } else {
     r.step = 2;
     r.off_b = 1;
-    return launch<T, 1, true>(r, head_dim, s);
+    return launch<T, 1, true>(r, p, s);
   }
 }
 
 template <typename T>
-hipError_t launch_type(RotaryArgs& r, int head_dim, bool half, int vec, hipStream_t s) {
+hipError_t launch_type(RotaryArgs& r, const Plan& p, bool half, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (vec == 8) return launch_layout<T, 8>(r, head_dim, half, s);
-  if (vec >= 4) return launch_layout<T, 4>(r, head_dim, half, s);
-  if (vec >= 2) return launch_layout<T, 2>(r, head_dim, half, s);
-  return launch_layout<T, 1>(r, head_dim, half, s);
+    if (p.vec == 8) return launch_layout<T, 8>(r, p, half, s);
+  if (p.vec >= 4) return launch_layout<T, 4>(r, p, half, s);
+  if (p.vec >= 2) return launch_layout<T, 2>(r, p, half, s);
+  return launch_layout<T, 1>(r, p, half, s);
 }
 }  // namespace
+
+int64_t rotary_threads(const f5hip_rotary_args& a) { return plan_of(a).threads; }
 
 hipError_t launch_rotary(const f5hip_rotary_args& a, hipStream_t s) {
   RotaryArgs r{};
@@ -200,21 +229,11 @@ hipError_t launch_rotary(const f5hip_rotary_args& a, hipStream_t s) {
   const auto same = [](const int64_t (&x)[3], const int64_t (&y)[3]) { return x[0] == y[0] && x[1] == y[1] && x[2] == y[2]; };
   r.keep_q = a.q == a.q_out && same(a.q_stride, a.q_out_stride);
   r.keep_k = a.k == a.k_out && same(a.k_stride, a.k_out_stride);
-  // The widest piece (16 bytes at most) that divides the rotated columns (their half in the half layout), the columns behind them, every
-  // stride and every pointer.
-  const int eb = a.dtype == F5HIP_T_FP32 ? 4 : 2;
+  const Plan p = plan_of(a);
+  if (p.threads > ROTARY_THREADS) return hipErrorInvalidValue;  // (the entry point says why)
+  r.npair = p.npair; r.nitem = p.nitem; r.hg = p.hg;
   const bool half = a.layout == F5HIP_ROTARY_HALF;
-  int vec = 16 / eb;
-  const auto fits = [&](int v) {
-    if ((half ? a.rot_dim / 2 : a.rot_dim) % v || (a.head_dim - a.rot_dim) % v) return false;
-    for (int i = 0; i < 3; ++i)
-      if (a.q_stride[i] % v || a.q_out_stride[i] % v || (a.heads_k && (a.k_stride[i] % v || a.k_out_stride[i] % v))) return false;
-    uintptr_t p = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out);
-    if (a.heads_k) p |= reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.k_out);
-    return p % (uintptr_t)(v * eb) == 0;
-  };
-  while (vec > 1 && !fits(vec)) vec /= 2;
-  if (a.dtype == F5HIP_T_FP16) return launch_type<f16>(r, a.head_dim, half, vec, s);
-  if (a.dtype == F5HIP_T_BF16) return launch_type<bf16>(r, a.head_dim, half, vec, s);
-  return launch_type<float>(r, a.head_dim, half, vec, s);
+  if (a.dtype == F5HIP_T_FP16) return launch_type<f16>(r, p, half, s);
+  if (a.dtype == F5HIP_T_BF16) return launch_type<bf16>(r, p, half, s);
+  return launch_type<float>(r, p, half, s);
 }

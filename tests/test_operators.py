@@ -295,6 +295,18 @@ def test_rotary_refuses_offsets_past_64_bits(operators_emu_lib):
         assert code == 1 and why in text, (kw, text)
 
 
+def test_rotary_refuses_more_threads_than_it_can_number(operators_emu_lib):
+    n, heads = 1 << 23, 32
+    big = dict(batch=1, tokens=n, heads_q=heads, inv_freq=1 << 50)
+    for odd in (2, 0):  # a pointer that is aligned to one element only: a piece is a pair
+        a = rotary_c(q=(1 << 40) + odd, q_out=(1 << 45) + odd, q_stride=[0, heads * 64, 64], q_out_stride=[0, heads * 64, 64], **big)
+        if odd:
+            code, text = refusal(operators_emu_lib, a)
+            assert code == 1 and "pieces" in text
+        else:  # 16-byte pieces: 2^30 threads are none too many (device 7 is one too many, so nothing is launched)
+            assert operators_emu_lib.f5hip_rotary(C.addressof(a), 7, None) == 1 and b"device" in operators_emu_lib.f5hip_last_error(None)
+
+
 def test_c_entries_refuse_null_and_say_why():
     lib = binding.load_library()
     assert lib.f5hip_rotary(None, 0, None) == 1 and b"null" in lib.f5hip_last_error(None)
