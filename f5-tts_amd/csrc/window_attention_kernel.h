@@ -13,10 +13,10 @@
 // three are below 2^-21 of it, below 2^-23 in the mean) on the bf16 matrix instructions, at 6 / 16 of the cost of the fp32 ones.  q is split once, K and V as
 // they are staged, P in registers.
 // Softmax.  exp2(c s - c m) with c = scale log2 e > 0 (a negative scale's sign is folded into q).  m is a reference, not the running maximum, and no
-// maximum is taken on the common path: the weights of a tile are summed anyway, and only where a lane's sum passes 2^15 — the reference is some 2^8 too
-// low, or none has been set — is the tile's maximum taken, O and l rescaled, and the tile's weights computed again.  The reference is set so that the
-// row's largest weight is 2^BIAS: in fp16 2^7, so that weights up to 2^15 are finite and those as small as 2^-21 of the largest are normal numbers,
-// rounded relative to themselves.
+// maximum is taken on the common path: the weights of a tile are summed anyway, and only where a lane's sum passes LIMIT = 2^(BIAS + 8) — the reference is
+// 2^3 to 2^8 too low, or none has been set — is the tile's maximum taken, O and l rescaled, and the tile's weights computed again.  The reference is set so
+// that the row's largest weight is 2^BIAS: in fp16 2^7, so that weights up to 2^15 are finite and those as small as 2^-21 of the largest are normal numbers,
+// rounded relative to themselves; in bf16 and fp32 1, and O, at most 2^8 |v| for every 16 keys, is finite where 16 |v| keys < 2^128.
 #pragma once
 #include <math.h>
 
@@ -45,7 +45,7 @@ template <typename T>
 struct Win;  // what differs between the element types
 template <>
 struct Win<f16> {
-  static constexpr float BIAS = 7.0f;
+  static constexpr float BIAS = 7.0f, LIMIT = 32768.0f;
   static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
@@ -57,7 +57,7 @@ struct Win<f16> {
 };
 template <>
 struct Win<bf16> {
-  static constexpr float BIAS = 0.0f;
+  static constexpr float BIAS = 0.0f, LIMIT = 256.0f;
   static __device__ __forceinline__ void mma(f32x16& c, const uint4& a, const uint4& b) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -161,7 +161,7 @@ struct Rows {
   static constexpr int EB = sizeof(T), PL = EB == 4 ? 3 : 1, ND = DP / 32, NKS = DP / 16;  // planes, blocks of 32 columns, steps of 16
   static constexpr int K_ROWB = DP * 2 + 16;            // of a plane in LDS: 32 rows read 16 bytes each without conflicts
   static constexpr int V_ROWB = DP == 64 ? 192 : 320;   // 4 rows start 64 bytes apart in the 256-byte bank row
-  static constexpr float UNSET = -3.402823466e38f, LIMIT = 32768.0f;
+  static constexpr float UNSET = -3.402823466e38f, LIMIT = Win<T>::LIMIT;
   f32x16 o[ND];
   float mc, l;  // c m - BIAS (UNSET: no key seen, any score passes the limit), this lane's share of the row sum
   int lo, hi;      // the lane's row: its window

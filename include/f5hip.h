@@ -329,7 +329,8 @@ int f5hip_rotary(const f5hip_rotary_args* args, int device, void* stream);
  * (negative: no bound; window_right = 0: causal; the sinks are exempt from the left bound only).  out = softmax(scale q . k) v over the
  * keys seen; a query that sees none gives zeros.  Query head h reads key head h / (heads / kv_heads).  Scores, softmax statistics and sums
  * are fp32; with 16-bit types the weights are rounded to that type for the product with v (the softmax sum is that of the rounded weights).
- * Scores have to stay below 2^22 in magnitude (an fp32 dot product of that size has lost the differences a softmax reads).
+ * Scores have to stay below 2^22 in magnitude (an fp32 dot product of that size has lost the differences a softmax reads), and 16 |v| times the keys
+ * that a query sees below 2^128 (the sums are divided at the end).
  * fp32 tensors are multiplied as three bf16 pieces a number, six products of nine: fp32 accuracy for finite numbers; an infinity that is seen gives
  * NaN.  `out` shares no element with q, k, v and the lengths, and has none twice: refused (it may lie between their rows or heads).
  *   kv_len, q_len   device int32 [batch] or NULL (kv_tokens / q_tokens), clamped into [0, kv_tokens] / [0, q_tokens].  Output rows

@@ -1,0 +1,23 @@
+"""GPU tests of the operators at the ends of their ranges (tests/operators_checks.py)."""
+import os
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+sys.path.insert(0, os.path.join(ROOT, "tests"))
+import operators_checks as K  # noqa: E402
+import operators_oracle as O  # noqa: E402
+from f5_tts_amd import ops  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+def gpu(t):
+    return t.cuda()
+
+
+def test_window_attention_of_large_values():
+    K.check_large_values(ops, gpu)

@@ -12,6 +12,7 @@ import torch
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 sys.path.insert(0, os.path.join(ROOT, "tests"))
+import operators_checks as K  # noqa: E402
 import operators_oracle as O  # noqa: E402
 from f5_tts_amd import binding, ops  # noqa: E402
 import hipemu_build  # noqa: E402
@@ -408,6 +409,11 @@ def test_writes_are_noticed_by_autograd_on_the_shim(host):
         y = x.clone()
         host.rotary(y, y.clone(), f, out=(y, torch.empty_like(y)))
         host.window_attention(y, y, y, out=torch.empty_like(y))
+
+
+@shim
+def test_window_attention_of_large_values_on_the_shim(host):
+    K.check_large_values(host, same)
 
 
 @shim
