@@ -191,7 +191,7 @@ const char* check_window_attention(const f5hip_window_attention_args& a) {
   if (a.head_dim < 1 || a.head_dim > 128 || (a.head_dim * eb) % 16) return "window attention: head_dim must be at most 128 and a whole multiple of 16 bytes";
   if (a.sinks < 0) return "window attention: sinks must be >= 0";
   if (a.align_end != 0 && a.align_end != 1) return "window attention: align_end must be 0 or 1";
-  if (!std::isfinite(a.scale)) return "window attention: scale must be finite";
+  if (!std::isfinite(a.scale * 1.4426950408889634f)) return "window attention: scale times log2(e) must be finite";  // (what the kernels multiply by)
   constexpr int lim = 1 << 30;  // sums of two of them stay in 32 bits
   if (a.q_tokens >= lim || a.kv_tokens >= lim || a.window_left >= lim || a.window_right >= lim || a.sinks >= lim)
     return "window attention: tokens, window and sinks must be below 2^30";

@@ -214,6 +214,14 @@ def test_overlaps_are_found_exactly_on_the_shim(host):
     assert min(said.values()) > 300
 
 
+def test_scales_that_overflow_are_refused(host):
+    x = q4(1, 4, 2, 64)
+    for scale in (3e38, -3e38, 2.4e38):  # 2^128 / log2(e) = 2.3587e38
+        with pytest.raises(ValueError, match="scale"):
+            host.window_attention(x, x, x, scale=scale)
+    host.window_attention(x, x, x, scale=2.3e38)
+
+
 def test_frequencies_that_require_a_gradient_are_refused(host):
     x, f = q4(1, 4, 2, 64), O.frequencies(64).requires_grad_()
     for layout in ("interleaved", "half"):
