@@ -9,9 +9,10 @@
 // round through LDS (eight angles a thread by itself cost 2000 cycles and 100 registers: 4 x 8192 tokens of 40 heads of 128 took 176 us; now 134 us,
 // 5.0 TB/s, which is what a large copy reaches on this card).
 //
-// The angle: turns t = p f / 2 pi in 64 bits, reduced to t - rint(t) in [-1/2, 1/2] in 64 bits (at p = 2^31 the product is 2^-22 turns exact),
-// then sin / cos of pi times twice that in fp32.  In fp32 from the start the product alone would be off by 2^-24 p f radians: 0.008 at
-// position 131 072.
+// The angle: p f turns by 1 / 2 pi, in units of a turn as p (w + e), w the 64-bit product f / 2 pi and e what its rounding and the constant's left behind.
+// p w less the nearest whole number is one fused operation, so for |p| up to 2^53 the turn, in [-1/2, 1/2], is that of the exact product to 2^-53, whatever
+// was reduced; then sin / cos of pi times twice that in fp32.  (In 64 bits without e it is off by 2^-22 turns at 2^31, in fp32 from the start by 2^-24 p f
+// radians: 0.008 at position 131 072.)
 #include <algorithm>
 
 #include "operators.h"
@@ -88,8 +89,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     for (int i = threadIdx.x; i < nangle; i += 256) {
       const int t = i / half_rot, f = i - t * half_rot;
       const int64_t tok = (int64_t)token0 + t, p = a.positions ? a.positions[(int64_t)b * a.position_stride + tok] : a.first + tok;
-      const double turns = (double)p * (a.inv_freq[f] * 0.15915494309189533577);  // 1 / 2 pi
-      const double r = turns - rint(turns);
+      constexpr double hi = 0x1.45f306dc9c883p-3, lo = -0x1.6b01ec5417056p-57;  // 1 / 2 pi
+      const double freq = a.inv_freq[f], w = freq * hi, e = fma(freq, lo, fma(freq, hi, -w)), at = (double)p;
+      const double r = fma(at, w, -rint(at * w)) + at * e;
       float2 cs;
 #ifdef F5_HIPEMU
       cs.x = (float)cos(6.283185307179586477 * r);

@@ -304,8 +304,9 @@ int f5hip_rotary_frequencies(int rot_dim, double base, int scaling, double facto
 /* replaces: apply_rotary_pos_emb on q and k (reference model/modules.py:498-509), whatever the layout of the pairs.
  * Token t of sequence b stands at p = positions[b * position_stride + t] (device int64; position_stride 0: one row for all sequences), or at
  * p = first + t where positions is NULL.  The pair (x, y) of frequency i becomes amplitude (x cos - y sin, x sin + y cos) of the angle
- * p inv_freq[i] (inverse != 0: minus the angle; the gradient of the operator).  The angle and its reduction are taken in 64 bits — exact to
- * fp32 rounding for |p| up to 2^31 and beyond —, the rotation in fp32, and each output is rounded once.  Columns >= rot_dim and, where rot_heads >= 0,
+ * p inv_freq[i] (inverse != 0: minus the angle; the gradient of the operator).  The angle is that of the exact product,
+ * reduced to half a turn, for |p| up to 2^53 (a position past that is rounded to 64-bit floating point first); it is rounded to fp32 then, the
+ * rotation is taken in fp32, and each output is rounded once.  Columns >= rot_dim and, where rot_heads >= 0,
  * heads >= rot_heads (of q and of k: the reference's pe_attn_head, modules.py:504-509) are copied.
  * An output may be its input (same pointer, same strides); any other element that an output shares with a buffer of the call, or has twice, is
  * refused (views whose elements lie between each other's are none of these).  heads_k = 0: q alone. */

@@ -1,4 +1,7 @@
 """More cases of the operators that the CPU (host shim) and GPU tests share; tests/operators_oracle.py has the definitions in 64 bits."""
+import math
+from fractions import Fraction
+
 import operators_oracle as O
 import torch
 
@@ -21,3 +24,45 @@ def check_large_values(ops, to):
                 want = v[0, 0, 0].double()
                 rel = 2 * (n + 16) * 2.0 ** -24 + 2.0 ** -22 + (O.half_step(t) if dtype == "bf16" else 0)
                 assert ((out - want).abs() <= rel * want.abs()).all(), (dtype, rows, n, above)
+
+
+def exact_turn(p, f):
+    """(cos, sin) of the angle p f, p a whole number and f a 64-bit float, both exact: reduced as a fraction of a turn with 1 / 2 pi to 400 bits."""
+    r = Fraction(p) * Fraction(f) * TURN
+    r = float(r - round(r))
+    return math.cos(2 * math.pi * r), math.sin(2 * math.pi * r)
+
+
+def _turn(bits=400):
+    def arctan_of_inverse(x):
+        total = term = (1 << bits) // x
+        n = 1
+        while term:
+            n, term = n + 2, -term // (x * x)
+            total += term // n
+        return total
+
+    # pi / 4 = 4 arctan(1 / 5) - arctan(1 / 239)
+    return Fraction(1 << bits, 8 * (4 * arctan_of_inverse(5) - arctan_of_inverse(239)))
+
+
+TURN = _turn()
+
+
+def check_far_positions(ops, to):
+    """Angles are those of the exact product up to 2^53: the fp32 terms of operators_oracle.rotary's bound, without one that grows with the position."""
+    far = [0, 1, -3, 131071, 2 ** 31 - 1, -2 ** 31, 2 ** 37 + 12345, 2 ** 40, -2 ** 45 + 7, 2 ** 50 + 1, 2 ** 53, -2 ** 53]
+    for rot, base in ((64, 10000.0), (8, 500000.0)):
+        f = O.frequencies(rot, base)
+        at = torch.tensor(far)
+        turns = [[exact_turn(p, float(x)) for x in f] for p in far]
+        c, s = (torch.tensor([[t[i] for t in row] for row in turns], dtype=torch.float64) for i in (0, 1))
+        x = torch.randn(1, len(far), 1, rot, generator=torch.Generator().manual_seed(3))
+        u, v = x.double()[0, :, 0, 0::2], x.double()[0, :, 0, 1::2]
+        size = (u.abs() + v.abs()) * (2.0 ** -22.3 + 2.0 ** -22 + 4 * 2.0 ** -24)
+        runs = [ops.rotary(to(x), None, to(f), positions=to(at))[0]]
+        runs.append(torch.cat([ops.rotary(to(x[:, i:i + 1]), None, to(f), offset=p)[0] for i, p in enumerate(far)], 1))
+        for y in runs:
+            y = y.cpu().double()[0, :, 0]
+            for got, want in ((y[:, 0::2], u * c - v * s), (y[:, 1::2], u * s + v * c)):
+                assert ((got - want).abs() <= size + 2.0 ** -24 * want.abs()).all(), rot

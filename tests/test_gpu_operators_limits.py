@@ -21,3 +21,7 @@ def gpu(t):
 
 def test_window_attention_of_large_values():
     K.check_large_values(ops, gpu)
+
+
+def test_rotary_of_far_positions():
+    K.check_far_positions(ops, gpu)

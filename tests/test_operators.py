@@ -420,6 +420,12 @@ def test_writes_are_noticed_by_autograd_on_the_shim(host):
 
 
 @shim
+def test_rotary_of_far_positions_on_the_shim(host):
+    assert abs(float(K.TURN) * 2 * math.pi - 1) < 2.0 ** -51
+    K.check_far_positions(host, same)
+
+
+@shim
 def test_window_attention_of_large_values_on_the_shim(host):
     K.check_large_values(host, same)
 
