@@ -66,3 +66,15 @@ def check_far_positions(ops, to):
             y = y.cpu().double()[0, :, 0]
             for got, want in ((y[:, 0::2], u * c - v * s), (y[:, 1::2], u * s + v * c)):
                 assert ((got - want).abs() <= size + 2.0 ** -24 * want.abs()).all(), rot
+
+
+# forms that operators_oracle.ATTENTION does not reach: 32 bits at up to 64 columns in 1024 and more blocks of 128 rows (32-key tiles in two stages),
+# few rows at 96 columns in fp32 and fp16, with one range of keys and with several
+MORE_ATTENTION = {
+    "fp32_many_blocks": (16, 140, 140, 32, 32, 64, "fp32", 30, 5, 9, "start", None, None),
+    "fp32_many_blocks_grouped": (9, 70, 90, 128, 64, 36, "fp32", 40, 3, 2, "end", [90 - 11 * i for i in range(9)], [70, 70, 1, 0, 33, 70, 64, 65, 2]),
+    "few_rows_fp32_96": (2, 1, 300, 6, 2, 96, "fp32", 250, 0, 9, "end", [300, 41], None),
+    "few_rows_fp16_96": (2, 3, 300, 6, 2, 96, "fp16", 250, 0, 9, "end", [300, 41], [3, 2]),
+    "few_rows_fp32_96_ranges": (1, 1, 1700, 4, 2, 96, "fp32", -1, 0, 0, "end", None, None),
+    "few_rows_fp16_72_ranges": (1, 2, 1700, 4, 2, 72, "fp16", 1600, 0, 3, "end", [1650], None),
+}

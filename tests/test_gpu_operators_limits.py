@@ -19,6 +19,12 @@ def gpu(t):
     return t.cuda()
 
 
+@pytest.mark.parametrize("name", sorted(K.MORE_ATTENTION))
+def test_more_window_attention(name):
+    O.check_attention(ops, gpu, K.MORE_ATTENTION[name], seed=8)
+    O.check_attention(ops, gpu, K.MORE_ATTENTION[name], seed=9, spread=30.0)
+
+
 def test_window_attention_of_large_values():
     K.check_large_values(ops, gpu)
 

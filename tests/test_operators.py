@@ -420,6 +420,12 @@ def test_writes_are_noticed_by_autograd_on_the_shim(host):
 
 
 @shim
+@pytest.mark.parametrize("name", sorted(K.MORE_ATTENTION))
+def test_more_window_attention_on_the_shim(host, name):
+    O.check_attention(host, same, K.MORE_ATTENTION[name], seed=8)
+
+
+@shim
 def test_rotary_of_far_positions_on_the_shim(host):
     assert abs(float(K.TURN) * 2 * math.pi - 1) < 2.0 ** -51
     K.check_far_positions(host, same)
