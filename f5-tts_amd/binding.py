@@ -120,7 +120,9 @@ def load_library(path: str = LIB_PATH) -> C.CDLL:
                          "there is no CPU fallback")
     lib = C.CDLL(path, mode=C.RTLD_GLOBAL)
     for name, (res, args) in SYMBOLS.items():
-        fn = getattr(lib, name)  # AttributeError if the .so does not export what the header declares
+        fn = getattr(lib, name, None)
+        if fn is None:  # (entry points may be added without a new ABI version)
+            raise F5HipError(f"{path} does not export {name}: it is older than this package — build it again (`make -C f5-tts_amd/csrc`)")
         fn.restype = res
         fn.argtypes = args
     if lib.f5hip_abi_version() != ABI_VERSION:

@@ -35,6 +35,9 @@
 extern "C" {
 #endif
 
+/* The version is raised where something that is there changes.  Entry points may be added within a version: rotary, window attention and the long form
+ * (f5hip_rotary*, f5hip_window_attention*, f5hip_set_long_form) came within v10, so a program that may meet an older v10 library looks them up
+ * (dlsym) before it calls them. */
 #define F5HIP_ABI_VERSION 10 /* v10: option "attn_stats" + f5hip_attention_stats; v9: option "mx_weights"; precision value 4 (a
                                 microbenchmark-only operand form of v8) removed */
 

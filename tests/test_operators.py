@@ -316,6 +316,12 @@ def test_rotary_refuses_more_threads_than_it_can_number(operators_emu_lib):
             assert operators_emu_lib.f5hip_rotary(C.addressof(a), 7, None) == 1 and b"device" in operators_emu_lib.f5hip_last_error(None)
 
 
+def test_a_library_without_the_operators_is_refused(operators_emu_lib):
+    """The operators came without a new ABI version, so their absence has to be said (here: a library that has them but not the engine)."""
+    with pytest.raises(binding.F5HipError, match="does not export"):
+        binding.load_library(operators_emu_lib._name)
+
+
 def test_c_entries_refuse_null_and_say_why():
     lib = binding.load_library()
     assert lib.f5hip_rotary(None, 0, None) == 1 and b"null" in lib.f5hip_last_error(None)
