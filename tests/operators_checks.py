@@ -78,3 +78,22 @@ MORE_ATTENTION = {
     "few_rows_fp32_96_ranges": (1, 1, 1700, 4, 2, 96, "fp32", -1, 0, 0, "end", None, None),
     "few_rows_fp16_72_ranges": (1, 2, 1700, 4, 2, 72, "fp16", 1600, 0, 3, "end", [1650], None),
 }
+
+
+def check_nan_keys(ops, to):
+    """A key that is NaN makes NaN of the rows that see it and touches no other, also those that share its tiles."""
+    for name in ("token_grouped", "three_tokens_odd_group", "chunk", "both_sides", "both_sides_bf16_128", "fp32_both_sides", "fp32_odd_dim", "causal"):
+        q, k, v, kw = O.attention_inputs(O.ATTENTION[name])
+        ref, tol, rows = O.attention(q, k, v, **kw)
+        n = k.shape[1] if kw["kv_len"] is None else int(kw["kv_len"][0])
+        j = n - 10 if kw["align"] == "end" else (2 * n) // 3  # (a key that some row sees)
+        k[0, j] = math.nan
+        out = ops.window_attention(to(q), to(k), to(v), **{x: to(y) if isinstance(y, torch.Tensor) else y for x, y in kw.items()}).cpu()
+        p = torch.arange(q.shape[1]) + (0 if kw["align"] == "start" else n - q.shape[1])
+        left, right = kw["window"]
+        sees = torch.ones(q.shape[1], dtype=torch.bool) if right < 0 else j <= p + right
+        if left >= 0:
+            sees = sees & ((j >= p - left) | (j < kw["sinks"]))
+        assert out[0, sees].isnan().all() and sees.any() and (name in ("token_grouped", "three_tokens_odd_group") or not sees.all()), name
+        out[0, sees] = ref[0, sees].to(out.dtype)
+        assert O.over(out, ref, tol) <= 1, name

@@ -29,5 +29,9 @@ def test_window_attention_of_large_values():
     K.check_large_values(ops, gpu)
 
 
+def test_window_attention_of_nan_keys():
+    K.check_nan_keys(ops, gpu)
+
+
 def test_rotary_of_far_positions():
     K.check_far_positions(ops, gpu)

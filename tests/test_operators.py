@@ -432,6 +432,11 @@ def test_more_window_attention_on_the_shim(host, name):
 
 
 @shim
+def test_window_attention_of_nan_keys_on_the_shim(host):
+    K.check_nan_keys(host, same)
+
+
+@shim
 def test_rotary_of_far_positions_on_the_shim(host):
     assert abs(float(K.TURN) * 2 * math.pi - 1) < 2.0 ** -51
     K.check_far_positions(host, same)
