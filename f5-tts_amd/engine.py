@@ -175,7 +175,8 @@ class F5HipEngine:
         """Sample long utterances through a sliding window (include/f5hip.h f5hip_set_long_form; DiT backbone): every frame attends to ``window``
         frames on both sides — an int, or ``(left, right)``; -1: no bound — and to the first ``sinks`` frames (the prompt's), with rotary frequencies
         scaled for utterances ``rope_factor`` times as long as the ``rope_original_length`` frames the model was trained on (``f5_tts_amd.ops.
-        rotary_frequencies``).  ``set_long_form()`` switches back to attention over the whole utterance."""
+        rotary_frequencies``).  ``set_long_form()`` switches back to attention over the whole utterance.  Faster in ``fp16`` and ``fp32``; ``fp16m`` and
+        ``fp16x3`` attend in fp32 meanwhile and get slower up to some 4096 frames."""
         if window is None and sinks:
             raise ValueError("sinks need a window: without one every frame attends to all of them")
         if window is None and rope_scaling is None:

@@ -180,7 +180,10 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     no bound on that side; ``right = 0``: causal) and, of the first ``sinks`` keys, all that ``right`` allows.  A query that sees no key gives
     zeros.  ``kv_len``, ``q_len``: valid keys and queries of each sequence; output rows behind ``q_len`` are zero, or left as they were in
     ``out``.  ``scale``: 1 / sqrt(D) by default.  D: a multiple of 8 (fp32: 4) up to 128.  Keys and values that no query sees may hold
-    anything, a value that some query sees has to be finite for the others' sake; tensors whose rows are not aligned to 16 bytes are copied first.  ``out`` shares no element with q, k and v."""
+    anything, a value that some query sees has to be finite for the others' sake; tensors whose rows are not aligned to 16 bytes are copied first.
+    Scaled scores have to stay below 2^22 in magnitude (past some 2^28 in fp16 and 2^32 in the others the result is NaN), and 16 |v| times the
+    keys of a query below 2^128.  In fp32 an infinity that a query sees gives NaN; in fp16 and bf16 a key that scores -inf has no weight.  ``out``
+    shares no element with q, k and v."""
     _tensor("q", q)
     dtype, where, shape = q.dtype, q.device, q.shape
     _tensor("k", k, dtype, where)

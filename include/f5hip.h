@@ -333,10 +333,11 @@ int f5hip_rotary(const f5hip_rotary_args* args, int device, void* stream);
  * (negative: no bound; window_right = 0: causal; the sinks are exempt from the left bound only).  out = softmax(scale q . k) v over the
  * keys seen; a query that sees none gives zeros.  Query head h reads key head h / (heads / kv_heads).  Scores, softmax statistics and sums
  * are fp32; with 16-bit types the weights are rounded to that type for the product with v (the softmax sum is that of the rounded weights).
- * Scores have to stay below 2^22 in magnitude (an fp32 dot product of that size has lost the differences a softmax reads), and 16 |v| times the keys
- * that a query sees below 2^128 (the sums are divided at the end).
+ * Scaled scores have to stay below 2^22 in magnitude (an fp32 dot product of that size has lost the differences a softmax reads; past some 2^28 in
+ * fp16 and 2^32 in the others the result is NaN), and 16 |v| times the keys that a query sees below 2^128 (the sums are divided at the end).
  * fp32 tensors are multiplied as three bf16 pieces a number, six products of nine: fp32 accuracy for finite numbers; an infinity that is seen gives
- * NaN.  `out` shares no element with q, k, v and the lengths, and has none twice: refused (it may lie between their rows or heads).
+ * NaN (in fp16 and bf16 a key that scores -inf has no weight, and only +inf gives NaN).
+ * `out` shares no element with q, k, v and the lengths, and has none twice: refused (it may lie between their rows or heads).
  *   kv_len, q_len   device int32 [batch] or NULL (kv_tokens / q_tokens), clamped into [0, kv_tokens] / [0, q_tokens].  Output rows
  *                   i >= q_len[b] are left as they were.  Keys at and past kv_len[b] and keys in front of every query's window are not
  *                   read, whatever they hold; a v row that SOME query of the call sees has to be finite for the others' sake.
@@ -360,7 +361,8 @@ int f5hip_window_attention(const f5hip_window_attention_args* args, int device, 
 /* Long utterances (the DiT backbone without qk_norm): from the next f5hip_sample on, the blocks' self-attention goes through the two operators above — each
  * frame attends to window_left frames before and window_right behind itself (-1: no bound) and to the first `sinks` frames (the prompt: pass its
  * frame count), positions rotate by frequencies scaled with rope_scaling (F5HIP_ROPE_*, factor, original length in frames: the longest the model was
- * trained on).  Attention then costs the window, not the square of the frames.  No counterpart in the reference, whose attention is always over the
+ * trained on).  Attention then costs the window, not the square of the frames — in fp32 in the split modes, which makes them slower up to some 4096
+ * frames.  No counterpart in the reference, whose attention is always over the
  * whole utterance (model/modules.py:511-520): with windows that hold every frame and no scaling the result is the ordinary one up to rounding.
  * precision: FP32, and FP16X3 / FP16M (whose block GEMMs then run as FP16X3), attend in fp32; FP16 in fp16.  Options "attn_impl", "attn_kv_split",
  * "attn_stats" and "packed_rows" have no effect meanwhile.  NULL: off (the default).  After f5hip_finalize_weights; synchronises the device. */
