@@ -4,6 +4,7 @@ import ctypes as C
 import math
 import os
 import random
+import subprocess
 import sys
 
 import pytest
@@ -316,10 +317,13 @@ def test_rotary_refuses_more_threads_than_it_can_number(operators_emu_lib):
             assert operators_emu_lib.f5hip_rotary(C.addressof(a), 7, None) == 1 and b"device" in operators_emu_lib.f5hip_last_error(None)
 
 
-def test_a_library_without_the_operators_is_refused(operators_emu_lib):
-    """The operators came without a new ABI version, so their absence has to be said (here: a library that has them but not the engine)."""
+def test_a_library_without_the_operators_is_refused(tmp_path):
+    """The operators came without a new ABI version, so their absence has to be said."""
+    (tmp_path / "old.c").write_text("int f5hip_abi_version_of_an_old_library(void) { return 10; }\n")
+    old = str(tmp_path / "libold.so")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", old, str(tmp_path / "old.c")], check=True)
     with pytest.raises(binding.F5HipError, match="does not export"):
-        binding.load_library(operators_emu_lib._name)
+        binding.load_library(old)
 
 
 def test_c_entries_refuse_null_and_say_why():
