@@ -177,8 +177,8 @@ const char* check_rotary(const f5hip_rotary_args& a) {
   const Runs freq(a.inv_freq, a.rot_dim / 2 * 8);
   Runs at(a.positions, (int64_t)a.tokens * 8);
   if (a.position_stride > 0) { at.n[0] = a.batch; at.stride[0] = a.position_stride * 8; }
-  for (const Runs* in : {&freq, (const Runs*)&at})
-    if (share_memory(qo, *in) || share_memory(ko, *in)) return "rotary: an output must share no memory with inv_freq and positions";
+  for (const Runs& in : {freq, at})
+    if (share_memory(qo, in) || share_memory(ko, in)) return "rotary: an output must share no memory with inv_freq and positions";
   if (rotary_threads(a) > ROTARY_THREADS) return "rotary: a sequence of more than 2^31 pieces (of up to 16 bytes, as alignment allows)";
   return nullptr;
 }
@@ -277,6 +277,11 @@ int f5hip_window_attention(const f5hip_window_attention_args* args, int device, 
   const int64_t need = window_attention_workspace(a);
   if (a.workspace_bytes < need || (need && (!a.workspace || !aligned(a.workspace, 16))))
     return f5hip_set_thread_error(F5HIP_ERR_INVALID, "window attention: workspace missing, too small or not aligned to 16 bytes");
+  const int64_t eq[3] = {a.batch, a.q_tokens, a.heads}, ek[3] = {a.batch, a.kv_tokens, a.kv_heads};
+  const int eb = elt_bytes(a.dtype);
+  for (const Runs& other : {Runs(a.out, a.head_dim, eb, a.out_stride, eq), Runs(a.q, a.head_dim, eb, a.q_stride, eq), Runs(a.k, a.head_dim, eb, a.k_stride, ek),
+                            Runs(a.v, a.head_dim, eb, a.v_stride, ek), Runs(a.kv_len, (int64_t)a.batch * 4), Runs(a.q_len, (int64_t)a.batch * 4)})
+    if (share_memory(Runs(a.workspace, need), other)) return f5hip_set_thread_error(F5HIP_ERR_INVALID, "window attention: the workspace must share no memory with the tensors");
   return on_device(device, [&] { return launch_window_attention(a, (hipStream_t)stream); });
 }
 }  // extern "C"

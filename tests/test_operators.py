@@ -317,6 +317,24 @@ def test_rotary_refuses_more_threads_than_it_can_number(operators_emu_lib):
             assert operators_emu_lib.f5hip_rotary(C.addressof(a), 7, None) == 1 and b"device" in operators_emu_lib.f5hip_last_error(None)
 
 
+def test_a_workspace_among_the_tensors_is_refused(operators_emu_lib):
+    lib, heads, n, d = operators_emu_lib, 4, 4000, 64
+    at = {"q": 1 << 40, "k": 1 << 41, "v": 1 << 42, "out": 1 << 43, "kv_len": 1 << 44, "q_len": 1 << 45}  # nobody's memory: no call is launched
+    st = [heads * d, heads * d, d, n * heads * d, heads * d, d, n * heads * d, heads * d, d, heads * d, heads * d, d]
+
+    def pack(work, size):
+        return ops._WINDOW.pack(1, 2, 1, n, heads, heads, d, -1, -1, 0, 0, 0.125, *(at[x] for x in ("q", "k", "v", "out")), *st, at["kv_len"], at["q_len"], work, size)
+
+    need = lib.f5hip_window_attention_workspace(pack(0, 0))
+    assert need > 0
+    ends = {"q": 2 * heads * d * 2, "k": 2 * n * heads * d * 2, "v": 2 * n * heads * d * 2, "out": 2 * heads * d * 2, "kv_len": 8, "q_len": 8}
+    for name, base in at.items():
+        for work in (base, base + (ends[name] - 1) // 16 * 16, base - need // 16 * 16 + 16):
+            assert lib.f5hip_window_attention(pack(work, need), 0, None) == 1 and b"share no memory" in lib.f5hip_last_error(None), (name, work)
+        after = base + (ends[name] + 15) // 16 * 16  # (device 7 is one too many, so nothing is launched)
+        assert lib.f5hip_window_attention(pack(after, need), 7, None) == 1 and b"device" in lib.f5hip_last_error(None), name
+
+
 def test_a_library_without_the_operators_is_refused(tmp_path):
     """The operators came without a new ABI version, so their absence has to be said."""
     (tmp_path / "old.c").write_text("int f5hip_abi_version_of_an_old_library(void) { return 10; }\n")
