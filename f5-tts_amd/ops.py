@@ -42,13 +42,15 @@ def _tensor(name: str, t: torch.Tensor, dtype: Optional[torch.dtype] = None, dev
             raise ValueError(f"{name}: {t.dtype} is not one of float32, float16, bfloat16")
     elif t.dtype != dtype or t.device != device:
         raise ValueError(f"{name}: {t.dtype} on {t.device}, the first tensor is {dtype} on {device}")
-    _inference(name, t)
+    if t.requires_grad or _forward_ad._current_level >= 0:
+        _inference(name, t)
 
 
 def _inference(name: str, t: torch.Tensor) -> None:
+    """Refuses what would lose a derivative.  Called where a tensor requires a gradient or a dual level is open (not -1)."""
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the operators are for inference (use torch.no_grad())")
-    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:  # (-1: no dual level is open)
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} carries a tangent of forward-mode differentiation: the operators are for inference (use its primal)")
 
 
@@ -103,8 +105,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, *
         raise ValueError(f"layout {layout!r}: 'interleaved' or 'half' is expected")
     if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != where:
         raise ValueError(f"inv_freq: a float64 vector on {where} is expected (rotary_frequencies)")
-    _inference("inv_freq", inv_freq)
-    if isinstance(amplitude, torch.Tensor):
+    if inv_freq.requires_grad or _forward_ad._current_level >= 0:
+        _inference("inv_freq", inv_freq)
+    if type(amplitude) is not float and isinstance(amplitude, torch.Tensor):
         _inference("amplitude", amplitude)
     inv_freq = inv_freq.contiguous()
     b, n, h, d = shape
@@ -194,7 +197,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
         raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}, v {tuple(v.shape)}: batch and head_dim must agree, k and v in all axes")
     if d == 0 or h == 0 or kshape[2] == 0:
         raise ValueError(f"q {tuple(shape)}, k {tuple(kshape)}: heads and head_dim must be positive")
-    if isinstance(scale, torch.Tensor):
+    if scale is not None and isinstance(scale, torch.Tensor):
         _inference("scale", scale)
     if align not in _ALIGN:
         raise ValueError(f"align {align!r}: 'start' or 'end' is expected")
